@@ -1,0 +1,55 @@
+// Norm over many gradient tensors: what its launcher hands to the kernels that clip by it (gradnorm.hip, optim.hip).
+#pragma once
+
+#include "gsr_common.h"
+
+namespace gsr {
+
+// Workgroups of one norm pass over all its launches, and so the partial results that every clipping wave joins again
+// (four or eight a lane).
+constexpr int kNormBlocks = 512;
+// Descriptors that fit one launch's kernel arguments (4 KB).
+constexpr int kGradsPerLaunch = 120;
+
+// Writes the partial results of all gradients to `partials` (norm_partials_most(count) doubles) and their number to
+// *used (0 when there is no element).  Arguments have been checked.
+int norm_partials(int count, const GsrGrad* h_grads, int norm_type, double* partials, int* used, hipStream_t stream);
+inline int norm_partials_most(int count) { return kNormBlocks + (count + kGradsPerLaunch - 1) / kGradsPerLaunch; }
+// GSR_OK if the list, the norm's type and the scratch are usable; the message names `what`.
+int check_norm(const char* what, int count, const GsrGrad* h_grads, int norm_type, const float* norm, const void* scratch,
+               size_t scratch_bytes);
+
+// Joins two partial results.  A maximum keeps a NaN once it has met one, as the sums do by themselves.
+template <int NORM>
+__device__ __forceinline__ double norm_join(double a, double b) {
+  if (NORM == GSR_NORM_MAX) return b > a || b != b ? b : a;
+  return a + b;
+}
+
+// Joins the 64 lanes' results; every lane gets the same bits (each step adds the same two numbers in both lanes).
+template <int NORM>
+__device__ __forceinline__ double norm_join_wave(double v) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) v = norm_join<NORM>(v, __shfl_xor(v, d));
+  return v;
+}
+
+// The norm from the partial results, by each wave for itself: no barrier, and the same order in every wave of a
+// launch, so that all of them clip by the same bits.
+template <int NORM>
+__device__ __forceinline__ double norm_of_partials(const double* __restrict__ partials, int used) {
+  double v = 0.0;
+  for (int i = threadIdx.x & 63; i < used; i += 64) v = norm_join<NORM>(v, partials[i]);
+  v = norm_join_wave<NORM>(v);
+  return NORM == GSR_NORM_2 ? sqrt(v) : v;
+}
+
+// min(1, max_norm / (norm + 1e-6)), the rule of torch.nn.utils.clip_grad_norm_: a NaN norm gives NaN, an infinite one 0.
+// An infinite bound never clips.
+__device__ __forceinline__ float clip_coefficient(double norm, double max_norm) {
+  if (max_norm == __builtin_inf()) return 1.0f;
+  const double c = max_norm / (norm + 1e-6);
+  return c < 1.0 || c != c ? (float)c : 1.0f;
+}
+
+}  // namespace gsr

@@ -1,0 +1,369 @@
+// Global norm over many gradient tensors, and clipping by it, on gfx950.
+//
+//     N = (sum_t sum_i |g_ti|^p)^(1/p)   p = 1, 2;   N = max |g_ti| for the maximum
+//     g <- g min(1, max_norm / (N + 1e-6))
+//
+// What bounds both is HBM: the norm reads every gradient once, clipping reads it once more and writes it only where
+// the coefficient is below 1.  One launch walks the tensors of a list (their descriptors are kernel arguments: nothing
+// is copied to the device, so a call can be captured into a graph); every workgroup leaves one partial result, and the
+// kernel that clips joins those by itself instead of waiting for a kernel that would.
+//
+// The sums are held in 64 bits: squares of the whole fp32 range neither overflow nor vanish, the result does not depend
+// on how many workgroups shared the work beyond its last bits, and the matrix-free fp64 rate of the card leaves the
+// kernel bound by memory all the same.
+#include "gradnorm.h"
+
+#include <algorithm>
+#include <new>
+
+namespace {
+
+using gsr::kGradsPerLaunch;
+using gsr::kNormBlocks;
+
+constexpr int kBlock = 512;
+constexpr int kRounds = 4;                                   // 16-byte accesses of a thread in flight
+constexpr uint32_t kChunk = kBlock * kRounds * 16;           // bytes
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// Tensors are cut into chunks at 16-byte boundaries of the address, so that every access inside is aligned whatever
+// the tensor's own alignment; its first and last vectors may be cut and go element by element.
+struct GradChunks {
+  struct One {
+    uintptr_t begin, end;
+    uint32_t first;                                          // number of its first chunk
+    uint32_t type;
+  } t[kGradsPerLaunch];
+  uint32_t chunks;
+  int count;
+};
+
+__device__ __forceinline__ float bf16_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
+__device__ __forceinline__ float f16_to_f32(uint32_t h) {
+  return (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+}
+// Rounded to nearest, ties to even; a NaN stays one.
+__device__ __forceinline__ uint32_t f32_to_bf16(float f) {
+  const uint32_t u = __float_as_uint(f);
+  if (f != f) return (u >> 16) | 0x40u;
+  return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
+__device__ __forceinline__ uint32_t f32_to_f16(float f) {
+  return (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)f);
+}
+
+template <int TYPE>
+struct Elem;
+template <>
+struct Elem<GSR_F32> {
+  static constexpr int kSize = 4;
+  __device__ static __forceinline__ float load(uintptr_t a) { return *(const float*)a; }
+  __device__ static __forceinline__ void store(uintptr_t a, float v) { *(float*)a = v; }
+};
+template <>
+struct Elem<GSR_F16> {
+  static constexpr int kSize = 2;
+  __device__ static __forceinline__ float load(uintptr_t a) { return f16_to_f32(*(const uint16_t*)a); }
+  __device__ static __forceinline__ void store(uintptr_t a, float v) { *(uint16_t*)a = (uint16_t)f32_to_f16(v); }
+};
+template <>
+struct Elem<GSR_BF16> {
+  static constexpr int kSize = 2;
+  __device__ static __forceinline__ float load(uintptr_t a) { return bf16_to_f32(*(const uint16_t*)a); }
+  __device__ static __forceinline__ void store(uintptr_t a, float v) { *(uint16_t*)a = (uint16_t)f32_to_bf16(v); }
+};
+
+template <int NORM>
+__device__ __forceinline__ double add(double acc, float x) {
+  const double d = (double)x;
+  if (NORM == GSR_NORM_2) return __builtin_fma(d, d, acc);
+  if (NORM == GSR_NORM_1) return acc + __builtin_fabs(d);
+  return gsr::norm_join<NORM>(acc, __builtin_fabs(d));
+}
+
+template <int NORM, int TYPE>
+__device__ __forceinline__ double add_word(double acc, uint32_t w) {
+  if (TYPE == GSR_F32) return add<NORM>(acc, __uint_as_float(w));
+  if (TYPE == GSR_F16) return add<NORM>(add<NORM>(acc, f16_to_f32(w & 0xffffu)), f16_to_f32(w >> 16));
+  return add<NORM>(add<NORM>(acc, __uint_as_float(w << 16)), __uint_as_float(w & 0xffff0000u));
+}
+
+template <int NORM, int TYPE>
+__device__ __forceinline__ double add_vector(double acc, u4 v) {
+  acc = add_word<NORM, TYPE>(acc, v.x);
+  acc = add_word<NORM, TYPE>(acc, v.y);
+  acc = add_word<NORM, TYPE>(acc, v.z);
+  return add_word<NORM, TYPE>(acc, v.w);
+}
+
+template <int NORM, int TYPE>
+__device__ __forceinline__ double add_chunk(double acc, uintptr_t base, uintptr_t begin, uintptr_t end) {
+  const uintptr_t mine = base + threadIdx.x * 16u;
+  if (base >= begin && base + kChunk <= end) {
+    u4 v[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; r++) v[r] = *(const u4*)(mine + (uintptr_t)r * kBlock * 16);
+#pragma unroll
+    for (int r = 0; r < kRounds; r++) acc = add_vector<NORM, TYPE>(acc, v[r]);
+    return acc;
+  }
+  for (int r = 0; r < kRounds; r++) {
+    const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
+    if (a >= end) break;
+    if (a >= begin && a + 16 <= end) {
+      acc = add_vector<NORM, TYPE>(acc, *(const u4*)a);
+    } else {
+      for (uintptr_t e = a < begin ? begin : a; e < a + 16 && e < end; e += Elem<TYPE>::kSize)
+        acc = add<NORM>(acc, Elem<TYPE>::load(e));
+    }
+  }
+  return acc;
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint32_t scale_word(uint32_t w, float c) {
+  if (TYPE == GSR_F32) return __float_as_uint(__uint_as_float(w) * c);
+  if (TYPE == GSR_F16) return f32_to_f16(f16_to_f32(w & 0xffffu) * c) | f32_to_f16(f16_to_f32(w >> 16) * c) << 16;
+  return f32_to_bf16(__uint_as_float(w << 16) * c) | f32_to_bf16(__uint_as_float(w & 0xffff0000u) * c) << 16;
+}
+
+template <int TYPE>
+__device__ __forceinline__ u4 scale_vector(u4 v, float c) {
+  const u4 o = {scale_word<TYPE>(v.x, c), scale_word<TYPE>(v.y, c), scale_word<TYPE>(v.z, c), scale_word<TYPE>(v.w, c)};
+  return o;
+}
+
+template <int TYPE>
+__device__ __forceinline__ void scale_chunk(float c, uintptr_t base, uintptr_t begin, uintptr_t end) {
+  const uintptr_t mine = base + threadIdx.x * 16u;
+  if (base >= begin && base + kChunk <= end) {
+    u4 v[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; r++) v[r] = *(const u4*)(mine + (uintptr_t)r * kBlock * 16);
+#pragma unroll
+    for (int r = 0; r < kRounds; r++) *(u4*)(mine + (uintptr_t)r * kBlock * 16) = scale_vector<TYPE>(v[r], c);
+    return;
+  }
+  for (int r = 0; r < kRounds; r++) {
+    const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
+    if (a >= end) break;
+    if (a >= begin && a + 16 <= end) {
+      *(u4*)a = scale_vector<TYPE>(*(const u4*)a, c);
+    } else {
+      for (uintptr_t e = a < begin ? begin : a; e < a + 16 && e < end; e += Elem<TYPE>::kSize)
+        Elem<TYPE>::store(e, Elem<TYPE>::load(e) * c);
+    }
+  }
+}
+
+// The tensor that chunk c lies in (the last whose first chunk is not behind it).
+__device__ __forceinline__ int tensor_of(const GradChunks& a, uint32_t c) {
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.t[mid].first <= c) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <int NORM>
+__global__ void __launch_bounds__(kBlock) norm_kernel(GradChunks a, double* __restrict__ partials) {
+  double acc = 0.0;
+  int k = tensor_of(a, blockIdx.x);
+  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+    while (k + 1 < a.count && a.t[k + 1].first <= c) k++;
+    const uintptr_t begin = a.t[k].begin, end = a.t[k].end;
+    const uintptr_t base = (begin & ~(uintptr_t)15) + (uintptr_t)(c - a.t[k].first) * kChunk;
+    switch (a.t[k].type) {
+      case GSR_F32: acc = add_chunk<NORM, GSR_F32>(acc, base, begin, end); break;
+      case GSR_F16: acc = add_chunk<NORM, GSR_F16>(acc, base, begin, end); break;
+      default: acc = add_chunk<NORM, GSR_BF16>(acc, base, begin, end); break;
+    }
+  }
+  __shared__ double s_wave[kBlock / 64];
+  acc = gsr::norm_join_wave<NORM>(acc);
+  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kBlock / 64; w++) acc = gsr::norm_join<NORM>(acc, s_wave[w]);
+    partials[blockIdx.x] = acc;
+  }
+}
+
+template <int NORM>
+__global__ void __launch_bounds__(64) norm_final_kernel(const double* __restrict__ partials, int used, float* __restrict__ norm) {
+  const double n = gsr::norm_of_partials<NORM>(partials, used);
+  if (threadIdx.x == 0) *norm = (float)n;
+}
+
+// Walks the chunks backwards: what the norm pass read last is still in the last-level cache.
+template <int NORM>
+__global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks a, const double* __restrict__ partials, int used,
+                                                      double max_norm, float* __restrict__ norm) {
+  const double n = gsr::norm_of_partials<NORM>(partials, used);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  const float coefficient = gsr::clip_coefficient(n, max_norm);
+  if (coefficient == 1.0f) return;                           // x * 1 is x: nothing to write
+  int k = tensor_of(a, a.chunks - 1 - blockIdx.x);
+  for (uint32_t i = blockIdx.x; i < a.chunks; i += gridDim.x) {
+    const uint32_t c = a.chunks - 1 - i;
+    while (a.t[k].first > c) k--;
+    const uintptr_t begin = a.t[k].begin, end = a.t[k].end;
+    const uintptr_t base = (begin & ~(uintptr_t)15) + (uintptr_t)(c - a.t[k].first) * kChunk;
+    switch (a.t[k].type) {
+      case GSR_F32: scale_chunk<GSR_F32>(coefficient, base, begin, end); break;
+      case GSR_F16: scale_chunk<GSR_F16>(coefficient, base, begin, end); break;
+      default: scale_chunk<GSR_BF16>(coefficient, base, begin, end); break;
+    }
+  }
+}
+
+inline size_t size_of(uint64_t type) { return type == GSR_F32 ? 4 : 2; }
+
+inline uint64_t chunks_of(const GsrGrad& g) {
+  if (!g.n) return 0;
+  const uintptr_t begin = (uintptr_t)g.grad;
+  return ((begin & 15) + g.n * size_of(g.type) + kChunk - 1) / kChunk;
+}
+
+// Descriptors of the next launch from h_grads[*at ..), empty tensors left out; advances *at.
+inline void fill(GradChunks& a, int count, const GsrGrad* h_grads, int* at) {
+  a.count = 0;
+  a.chunks = 0;
+  for (; *at < count && a.count < kGradsPerLaunch; ++*at) {
+    const GsrGrad& g = h_grads[*at];
+    const uint64_t chunks = chunks_of(g);
+    if (!chunks) continue;
+    const uintptr_t begin = (uintptr_t)g.grad;
+    a.t[a.count++] = {begin, begin + g.n * size_of(g.type), a.chunks, (uint32_t)g.type};
+    a.chunks += (uint32_t)chunks;
+  }
+}
+
+}  // namespace
+
+namespace gsr {
+
+int check_norm(const char* what, int count, const GsrGrad* h_grads, int norm_type, const float* norm, const void* scratch,
+               size_t scratch_bytes) {
+  GSR_REQUIRE(count >= 0, "%s: %d tensors", what, count);
+  GSR_REQUIRE(count == 0 || h_grads, "%s: null tensor list", what);
+  GSR_REQUIRE(norm_type == GSR_NORM_MAX || norm_type == GSR_NORM_1 || norm_type == GSR_NORM_2, "%s: norm type %d", what,
+              norm_type);
+  GSR_REQUIRE(norm, "%s: null pointer for the norm", what);
+  uint64_t chunks = 0;
+  for (int k = 0; k < count; k++) {
+    const GsrGrad& g = h_grads[k];
+    GSR_REQUIRE(g.type == GSR_F32 || g.type == GSR_F16 || g.type == GSR_BF16, "%s: tensor %d has unknown type %llu", what, k,
+                (unsigned long long)g.type);
+    if (!g.n) continue;
+    GSR_REQUIRE(g.grad, "%s: null pointer in tensor %d", what, k);
+    GSR_REQUIRE((uintptr_t)g.grad % size_of(g.type) == 0, "%s: tensor %d is not aligned to its elements", what, k);
+    GSR_REQUIRE(g.n <= ((size_t)1 << 44), "%s: tensor %d has %zu elements", what, k, g.n);
+    chunks += chunks_of(g);
+  }
+  GSR_REQUIRE(chunks < ((uint64_t)1 << 31), "%s: %llu chunks of gradients", what, (unsigned long long)chunks);
+  if (scratch_bytes < gsr_grad_norm_bytes(count))
+    return fail(GSR_E_SCRATCH, "%s: scratch too small: %zu of %zu bytes", what, scratch_bytes, gsr_grad_norm_bytes(count));
+  if (!scratch || ((uintptr_t)scratch & 255)) return fail(GSR_E_SCRATCH, "%s: scratch must be 256-byte aligned", what);
+  return GSR_OK;
+}
+
+int norm_partials(int count, const GsrGrad* h_grads, int norm_type, double* partials, int* used, hipStream_t stream) {
+  uint64_t total = 0;
+  for (int k = 0; k < count; k++) total += chunks_of(h_grads[k]);
+  *used = 0;
+  GradChunks a;
+  for (int at = 0; at < count;) {
+    fill(a, count, h_grads, &at);
+    if (!a.chunks) continue;
+    // each launch gets its share of the workgroups, rounded up: at most one more per launch in all
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(a.chunks, ((uint64_t)kNormBlocks * a.chunks + total - 1) / total);
+    double* out = partials + *used;
+    if (norm_type == GSR_NORM_2) hipLaunchKernelGGL(norm_kernel<GSR_NORM_2>, dim3(blocks), dim3(kBlock), 0, stream, a, out);
+    else if (norm_type == GSR_NORM_1) hipLaunchKernelGGL(norm_kernel<GSR_NORM_1>, dim3(blocks), dim3(kBlock), 0, stream, a, out);
+    else hipLaunchKernelGGL(norm_kernel<GSR_NORM_MAX>, dim3(blocks), dim3(kBlock), 0, stream, a, out);
+    const int rc = check_launch("grad_norm");
+    if (rc != GSR_OK) return rc;
+    *used += (int)blocks;
+  }
+  return GSR_OK;
+}
+
+}  // namespace gsr
+
+namespace {
+
+int write_norm(const double* partials, int used, int norm_type, float* norm, hipStream_t stream) {
+  if (norm_type == GSR_NORM_2) hipLaunchKernelGGL(norm_final_kernel<GSR_NORM_2>, dim3(1), dim3(64), 0, stream, partials, used, norm);
+  else if (norm_type == GSR_NORM_1) hipLaunchKernelGGL(norm_final_kernel<GSR_NORM_1>, dim3(1), dim3(64), 0, stream, partials, used, norm);
+  else hipLaunchKernelGGL(norm_final_kernel<GSR_NORM_MAX>, dim3(1), dim3(64), 0, stream, partials, used, norm);
+  return gsr::check_launch("grad_norm");
+}
+
+// Whether two tensors of the list share memory (each would be scaled by its own workgroups, in any order).
+// -1 without the memory to find out.
+int any_overlap(int count, const GsrGrad* h_grads) {
+  struct Span { uintptr_t begin, end; };
+  Span few[64];
+  Span* spans = count <= 64 ? few : new (std::nothrow) Span[count];
+  if (!spans) return -1;
+  int n = 0;
+  for (int k = 0; k < count; k++) {
+    const uintptr_t begin = (uintptr_t)h_grads[k].grad;
+    if (h_grads[k].n) spans[n++] = {begin, begin + h_grads[k].n * size_of(h_grads[k].type)};
+  }
+  std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  int found = 0;
+  for (int k = 1; k < n; k++) found |= spans[k].begin < spans[k - 1].end;
+  if (spans != few) delete[] spans;
+  return found;
+}
+
+}  // namespace
+
+extern "C" size_t gsr_grad_norm_bytes(int count) {
+  return gsr::align_up((size_t)gsr::norm_partials_most(count > 0 ? count : 0) * sizeof(double), 256);
+}
+
+extern "C" int gsr_grad_norm(int count, const GsrGrad* h_grads, int norm_type, float* norm, void* scratch,
+                             size_t scratch_bytes, void* stream) {
+  int rc = gsr::check_norm("grad_norm", count, h_grads, norm_type, norm, scratch, scratch_bytes);
+  if (rc != GSR_OK) return rc;
+  int used = 0;
+  rc = gsr::norm_partials(count, h_grads, norm_type, (double*)scratch, &used, (hipStream_t)stream);
+  if (rc != GSR_OK) return rc;
+  return write_norm((const double*)scratch, used, norm_type, norm, (hipStream_t)stream);
+}
+
+extern "C" int gsr_clip_grads(int count, const GsrGrad* h_grads, int norm_type, double max_norm, float* norm, void* scratch,
+                              size_t scratch_bytes, void* stream) {
+  int rc = gsr::check_norm("clip_grads", count, h_grads, norm_type, norm, scratch, scratch_bytes);
+  if (rc != GSR_OK) return rc;
+  GSR_REQUIRE(max_norm >= 0.0, "clip_grads: bound %g", max_norm);
+  const int overlap = any_overlap(count, h_grads);
+  GSR_REQUIRE(overlap >= 0, "clip_grads: no memory to compare %d tensors", count);
+  GSR_REQUIRE(!overlap, "clip_grads: two tensors of the list share memory");
+  double* partials = (double*)scratch;
+  int used = 0;
+  rc = gsr::norm_partials(count, h_grads, norm_type, partials, &used, (hipStream_t)stream);
+  if (rc != GSR_OK) return rc;
+  if (used == 0) return write_norm(partials, 0, norm_type, norm, (hipStream_t)stream);
+  GradChunks a;
+  for (int at = 0; at < count;) {
+    fill(a, count, h_grads, &at);
+    if (!a.chunks) continue;
+    const uint32_t blocks = std::min<uint32_t>(a.chunks, kNormBlocks * 2);
+    if (norm_type == GSR_NORM_2)
+      hipLaunchKernelGGL(clip_kernel<GSR_NORM_2>, dim3(blocks), dim3(kBlock), 0, (hipStream_t)stream, a, partials, used, max_norm, norm);
+    else if (norm_type == GSR_NORM_1)
+      hipLaunchKernelGGL(clip_kernel<GSR_NORM_1>, dim3(blocks), dim3(kBlock), 0, (hipStream_t)stream, a, partials, used, max_norm, norm);
+    else
+      hipLaunchKernelGGL(clip_kernel<GSR_NORM_MAX>, dim3(blocks), dim3(kBlock), 0, (hipStream_t)stream, a, partials, used, max_norm, norm);
+    rc = gsr::check_launch("clip_grads");
+    if (rc != GSR_OK) return rc;
+    norm = nullptr;                                          // the first launch has written it
+  }
+  return GSR_OK;
+}

@@ -14,7 +14,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 from dataclasses import dataclass
-from typing import Dict, List, Optional
+from typing import Dict, Iterable, List, Optional, Union
 
 import torch
 import torch.distributed as dist
@@ -32,6 +32,16 @@ class _AdamTensor(C.Structure):
 
 _lib.gsr_adam_step.argtypes = [C.c_int, C.POINTER(_AdamTensor), C.c_double, C.c_double, C.c_double, C.c_int, C.c_float,
                                C.c_void_p]
+_lib.gsr_grad_norm_bytes.restype = C.c_size_t
+_lib.gsr_grad_norm_bytes.argtypes = [C.c_int]
+_lib.gsr_grad_norm.argtypes = [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+_lib.gsr_clip_grads.argtypes = [C.c_int, C.c_void_p, C.c_int, C.c_double, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+_lib.gsr_adam_step_clipped.argtypes = [C.c_int, C.POINTER(_AdamTensor), C.POINTER(C.c_int), C.c_double, C.c_double, C.c_double,
+                                       C.c_int, C.c_float, C.c_int, C.c_double, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t,
+                                       C.c_void_p]
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}         # GSR_F32, GSR_F16, GSR_BF16 of gsr.h
+_NORMS = {math.inf: 0, 1.0: 1, 2.0: 2}                                   # GSR_NORM_MAX, GSR_NORM_1, GSR_NORM_2
+Grads = Union[torch.Tensor, Iterable[Optional[torch.Tensor]], Dict[str, Optional[torch.Tensor]]]
 
 
 def expon_lr(step: int, lr_init: float, lr_final: float, lr_delay_steps: int = 0, lr_delay_mult: float = 1.0,
@@ -125,6 +135,15 @@ class GradArena:
     def zero_(self) -> None:
         self.flat.zero_()
 
+    def norm(self, norm_type: float = 2.0) -> torch.Tensor:
+        """``grad_norm`` of all gradients, as one stretch of memory (the padding is zero).  After ``all_reduce``: every
+        rank then holds the same gradients and finds the same norm, without a collective of its own."""
+        return grad_norm(self.flat, norm_type)
+
+    def clip_(self, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+        """``clip_grads_`` of all gradients; after ``all_reduce``, as ``norm``."""
+        return clip_grads_(self.flat, max_norm, norm_type)
+
     def all_reduce(self, group=None, average: bool = True, method: str = "scatter_gather") -> float:
         """Sums the gradients over the ranks of ``group`` (``method``: see _sum_flat_over_ranks; two collectives on
         the one flat buffer by default) and returns the factor the
@@ -176,6 +195,108 @@ def all_reduce_gradients(params: Dict[str, torch.Tensor], group=None, average: b
         for w in pending:
             w.wait()
     return 1.0 / world if average else 1.0
+
+
+def _norm_code(norm_type: float) -> int:
+    code = _NORMS.get(float(norm_type))
+    if code is None:
+        raise ValueError(f"norm_type must be 1, 2 or infinity, got {norm_type}")
+    return code
+
+
+def _grad_list(grads: Grads) -> List[torch.Tensor]:
+    """The tensors of ``grads``, checked: on one GPU, of a type the kernels read."""
+    if isinstance(grads, torch.Tensor):
+        grads = (grads,)
+    elif isinstance(grads, dict):
+        grads = grads.values()
+    out = [g for g in grads if g is not None]
+    if not out:
+        raise ValueError("no gradients given")
+    dev = out[0].device
+    for g in out:
+        if g.dtype not in _TYPES:
+            raise TypeError(f"gradients must be float32, float16 or bfloat16, got {g.dtype}")
+        if not g.is_cuda or g.layout != torch.strided:
+            raise ValueError(f"gradients must be dense tensors on the GPU, got {g.layout} on {g.device}")
+        if g.device != dev:
+            raise ValueError(f"gradients are on {dev} and {g.device}: one call works on one GPU")
+    return out
+
+
+def _fills_its_memory(t: torch.Tensor) -> bool:
+    """Whether the elements, in whatever order of dimensions, fill one stretch of memory without gaps."""
+    if t.is_contiguous():
+        return True
+    order = sorted(range(t.dim()), key=lambda d: (t.stride(d), t.size(d)), reverse=True)
+    return t.permute(order).is_contiguous()
+
+
+def _shares_elements(t: torch.Tensor) -> bool:
+    """Whether two elements may lie at one address (an expanded tensor, or one of overlapping windows)."""
+    reach = 0
+    for stride, size in sorted((t.stride(d), t.size(d)) for d in range(t.dim()) if t.size(d) > 1):
+        if stride <= reach:
+            return True
+        reach += (size - 1) * stride
+    return False
+
+
+def _run_norm(what: str, fn, tensors: List[torch.Tensor], code: int, *bound: float) -> torch.Tensor:
+    """One norm or clipping call over tensors that fill their memory, on the current stream of their GPU."""
+    dev = tensors[0].device
+    with torch.cuda.device(dev):
+        words: List[int] = []
+        for g in tensors:
+            words += (g.data_ptr(), g.numel(), _TYPES[g.dtype])
+        n = len(tensors)
+        nb = _lib.gsr_grad_norm_bytes(n)
+        scratch = torch.empty((nb,), dtype=torch.uint8, device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        _dgr._run(what, fn, n, (C.c_uint64 * (3 * n))(*words), code, *bound, _dgr._ptr(norm), _dgr._ptr(scratch), nb,
+                  _dgr._stream())
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all gradients together, as a float32 scalar on their GPU; nothing waits for it.
+
+    ``grads``: a tensor, an iterable or a dictionary of tensors (entries that are None are left out), float32, float16
+    and bfloat16 mixed as they come, of any shape and strides.  ``norm_type``: 2 (root of the sum of squares), 1 (sum
+    of magnitudes) or infinity (the largest magnitude).  Sums are held in 64 bits; a NaN anywhere gives NaN.
+    A tensor that is given twice counts twice."""
+    tensors = [g if _fills_its_memory(g) else g.contiguous() for g in _grad_list(grads)]
+    return _run_norm("grad_norm", _lib.gsr_grad_norm, tensors, _norm_code(norm_type))
+
+
+@torch.no_grad()
+def clip_grads_(grads: Grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """Scales all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` (the rule of
+    ``torch.nn.utils.clip_grad_norm_``) and returns the norm they had, a float32 scalar on their GPU.
+
+    Arguments as ``grad_norm``'s; two tensors that share memory, or one that shares it with itself (expanded), are
+    refused.  The product is formed in float32 and rounded once.  A NaN norm makes every element NaN and an infinite
+    one the finite elements 0, as there: look at the returned norm, or let ``GaussianAdam.step(skip_nonfinite=True)``.
+    An infinite ``max_norm`` scales nothing."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be at least 0, got {max_norm}")
+    code, tensors = _norm_code(norm_type), _grad_list(grads)
+    direct, staged = [], []
+    for g in tensors:
+        if _fills_its_memory(g):
+            direct.append(g)
+        elif _shares_elements(g):
+            raise ValueError(f"a gradient of shape {tuple(g.shape)} and strides {g.stride()} has elements that share memory")
+        else:
+            staged.append((g, g.contiguous()))
+            direct.append(staged[-1][1])
+    norm = _run_norm("clip_grads", _lib.gsr_clip_grads, direct, code, max_norm)
+    for g, scaled in staged:
+        g.copy_(scaled)
+    torch.autograd.graph.increment_version(tensors)          # written behind autograd's back
+    return norm
 
 
 class GaussianAdam:
@@ -302,28 +423,63 @@ class GaussianAdam:
             self.betas, self.eps = tuple(groups[0]["betas"]), float(groups[0]["eps"])
 
     @torch.no_grad()
-    def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_scale: float = 1.0) -> None:
-        """One Adam update of every tensor that has a gradient (``grads[name]`` or ``param.grad``)."""
+    def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_scale: float = 1.0,
+             max_norm: Optional[float] = None, norm_type: float = 2.0, skip_nonfinite: bool = False) -> Optional[torch.Tensor]:
+        """One Adam update of every tensor that has a gradient (``grads[name]`` or ``param.grad``).
+
+        With ``max_norm`` the norm of all gradients of the step, after ``grad_scale``, is bounded first, as
+        ``clip_grads_`` would (``norm_type`` as there), in the same two launches and without touching the gradients,
+        which may then be float32, float16 or bfloat16; the step returns the norm, a float32 scalar on the GPU.
+        ``max_norm=math.inf`` only measures.  ``skip_nonfinite`` (with ``max_norm``): a step whose norm is infinite or
+        NaN leaves parameters and moments as they are; ``step_count`` counts it."""
         for name, p in self.params.items():
             if not p.is_cuda:
                 raise ValueError(f"{name}: the fused update runs on the GPU only, the parameter is on {p.device}")
-        self.step_count += 1
-        arr = (_AdamTensor * MAX_TENSORS)()
+        if max_norm is None:
+            if skip_nonfinite:
+                raise ValueError("skip_nonfinite needs max_norm: a step without it does not look at the gradients first")
+        else:
+            max_norm, code = float(max_norm), _norm_code(norm_type)
+            if not max_norm >= 0.0:
+                raise ValueError(f"max_norm must be at least 0, got {max_norm}")
+        arr, types = (_AdamTensor * MAX_TENSORS)(), (C.c_int * MAX_TENSORS)()
         n = 0
+        dev = next(iter(self.params.values())).device if self.params else torch.device("cuda")
         keep: List[torch.Tensor] = []
         for name, p in self.params.items():
             g = grads[name] if grads is not None else p.grad
             if g is None:
                 continue
-            g = _dgr._f32(g, f"grad of {name}")
             if g.numel() != p.numel():
                 raise ValueError(f"{name}: gradient has {g.numel()} elements, parameter {p.numel()}")
+            if g.numel() == 0:
+                continue
+            if max_norm is None:
+                g = _dgr._f32(g, f"grad of {name}")
+            else:
+                if g.dtype not in _TYPES:
+                    raise TypeError(f"grad of {name} must be float32, float16 or bfloat16, got {g.dtype}")
+                if g.device != dev or p.device != dev:
+                    raise ValueError(f"{name}: parameter and gradient must be on {dev}, they are on {p.device} and {g.device}")
+                types[n] = _TYPES[g.dtype]
+                g = g.contiguous()
             keep.append(g)
             arr[n] = _AdamTensor(p.data_ptr(), g.data_ptr(), self.exp_avg[name].data_ptr(),
                                  self.exp_avg_sq[name].data_ptr(), p.numel(), float(self.lrs[name]), 0)
             n += 1
-        _dgr._run("adam_step", _lib.gsr_adam_step, n, arr, float(self.betas[0]), float(self.betas[1]),
-                  float(self.eps), int(self.step_count), float(grad_scale), _dgr._stream())
+        self.step_count += 1
+        if max_norm is None:
+            _dgr._run("adam_step", _lib.gsr_adam_step, n, arr, float(self.betas[0]), float(self.betas[1]),
+                      float(self.eps), int(self.step_count), float(grad_scale), _dgr._stream())
+            return None
+        with torch.cuda.device(dev):
+            nb = _lib.gsr_grad_norm_bytes(n)
+            scratch = torch.empty((nb,), dtype=torch.uint8, device=dev)
+            norm = torch.empty((), dtype=torch.float32, device=dev)
+            _dgr._run("adam_step", _lib.gsr_adam_step_clipped, n, arr, types, float(self.betas[0]), float(self.betas[1]),
+                      float(self.eps), int(self.step_count), float(grad_scale), code, max_norm, int(bool(skip_nonfinite)),
+                      _dgr._ptr(norm), _dgr._ptr(scratch), nb, _dgr._stream())
+        return norm
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         """train.py:128."""

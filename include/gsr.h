@@ -506,6 +506,55 @@ typedef struct GsrAdamTensor {
 int gsr_adam_step(int count, const GsrAdamTensor* h_tensors, double beta1, double beta2, double eps,
                   int step, float grad_scale, void* stream);
 
+/* ---- Gradient norm and clipping ----------------------------------------------
+ * What stands between the backward and the step of a training loop that bounds its
+ * gradients (the reference's loop has neither; its place there would be between
+ * train.py:92 and :126).  h_grads is a HOST array of `count` descriptors, any number of
+ * them; tensors may have any length (0 included), type and alignment (of their elements),
+ * types may be mixed.
+ * gsr_grad_norm: *norm (device) = the norm of all elements together: GSR_NORM_2 the
+ * root of the sum of squares, GSR_NORM_1 the sum of magnitudes, GSR_NORM_MAX the largest
+ * magnitude; 0 without elements, NaN if any element is NaN.  Sums are held in 64 bits;
+ * their order depends on the sizes and alignments only, so equal calls give equal bits.
+ * gsr_clip_grads: the same norm, and every element times min(1, max_norm / (norm + 1e-6)),
+ * the factor and the product in fp32 and the product rounded to its type (the rule of
+ * torch.nn.utils.clip_grad_norm_: a NaN norm makes every element NaN, an infinite one makes
+ * infinite elements NaN and the others 0).  The factor comes from the 64-bit norm, so it is
+ * right where the fp32 *norm overflows.  max_norm >= 0; infinity never scales.  Nothing is
+ * written where the factor is 1.  Tensors of the list that share memory are refused.
+ * scratch: gsr_grad_norm_bytes(count) bytes, its contents do not matter. */
+#define GSR_F32 0
+#define GSR_F16 1
+#define GSR_BF16 2
+#define GSR_NORM_MAX 0
+#define GSR_NORM_1 1
+#define GSR_NORM_2 2
+typedef struct GsrGrad {
+  void* grad;
+  size_t n;      /* elements */
+  uint64_t type; /* GSR_F32, GSR_F16 or GSR_BF16 */
+} GsrGrad;
+size_t gsr_grad_norm_bytes(int count);
+int gsr_grad_norm(int count, const GsrGrad* h_grads, int norm_type, float* norm, void* scratch,
+                  size_t scratch_bytes, void* stream);
+int gsr_clip_grads(int count, const GsrGrad* h_grads, int norm_type, double max_norm, float* norm,
+                   void* scratch, size_t scratch_bytes, void* stream);
+
+/* gsr_adam_step with the gradients' norm bounded first: the update from
+ * grad * grad_scale * min(1, max_norm / (norm + 1e-6)), *norm (device) = the norm of
+ * grad * grad_scale over all tensors of the call, as gsr_clip_grads has it; the gradients
+ * themselves stay as they are.  While the norm is within the bound the results are
+ * gsr_adam_step's, bit for bit.
+ * h_grad_types: the type behind each tensor's `grad` pointer (GSR_F32, GSR_F16,
+ * GSR_BF16), NULL = all fp32; parameters and moments are fp32 always.
+ * skip_nonfinite != 0: a step whose norm is infinite or NaN changes nothing (`step`
+ * counts it all the same: the caller's bias corrections run on).
+ * scratch: gsr_grad_norm_bytes(count). */
+int gsr_adam_step_clipped(int count, const GsrAdamTensor* h_tensors, const int* h_grad_types,
+                          double beta1, double beta2, double eps, int step, float grad_scale,
+                          int norm_type, double max_norm, int skip_nonfinite, float* norm,
+                          void* scratch, size_t scratch_bytes, void* stream);
+
 /* ---- Initial scales: mean squared distance to the three nearest neighbours ----
  * distCUDA2 of the reference's second native submodule, simple_knn (call site
  * scene/gaussian_model.py:134, used once, to initialise the scales; the
