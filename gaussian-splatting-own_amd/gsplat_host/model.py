@@ -11,7 +11,8 @@ densification statistics fed by the rasterizer's screen-space gradient
 host bookkeeping that changes the number of Gaussians between steps
 (``:120-122, 179-189, 291-403``: SH degree ramp, opacity reset, and the clone / split /
 prune refinement as one pass) with the checkpoint tuple (``:61-93``), all on top of ``GaussianAdam``'s
-state surgery.  These are plain PyTorch tensor operations, as in the reference.
+state surgery.  Which Gaussians go and where the new ones come from are plain PyTorch tensor operations, as in the
+reference; on the GPU the rows themselves are moved by ``gsplat_host.rows``.
 """
 from __future__ import annotations
 
@@ -122,9 +123,13 @@ class GaussianParams(nn.Module):
         """:291-305: removes the Gaussians selected by ``mask``."""
         keep = ~mask
         self._adopt(self.optimizer.prune(keep))
-        self.xyz_gradient_accum = self.xyz_gradient_accum[keep]
-        self.denom = self.denom[keep]
-        self.max_radii2D = self.max_radii2D[keep]
+        stats = (self.xyz_gradient_accum, self.denom, self.max_radii2D)
+        if keep.is_cuda and all(t.device == keep.device for t in stats):
+            from .rows import compact_rows
+            stats, _ = compact_rows(stats, keep)
+        else:
+            stats = [t[keep] for t in stats]
+        self.xyz_gradient_accum, self.denom, self.max_radii2D = stats
 
     def densification_postfix(self, new_xyz, new_features_dc, new_features_rest, new_opacities, new_scaling,
                               new_rotation) -> None:
@@ -167,25 +172,35 @@ class GaussianParams(nn.Module):
         spread = scale[family]
         offsets = torch.randn(spread.shape, generator=generator, device=generator.device if generator else dev).to(dev) * spread
         world = torch.einsum("nij,nj->ni", quaternion_to_matrix(self._rotation[family]), offsets)
-        born = {"xyz": torch.cat((self._xyz[copy_idx], self._xyz[family] + world)),
-                "scaling": torch.cat((self._scaling[copy_idx], torch.log(spread / (0.8 * children))))}
-        for group, attr in self.GROUPS:
-            if group not in born:
-                t = getattr(self, attr)
-                born[group] = torch.cat((t[copy_idx], t[family]))
-        appended = copy_idx.numel() + family.numel()
-        if appended:
-            self.densification_postfix(born["xyz"], born["f_dc"], born["f_rest"], born["opacity"], born["scaling"],
-                                       born["rotation"])
+        source = torch.cat((copy_idx, family))
+        tensors = [getattr(self, attr).detach() for _, attr in self.GROUPS]
+        if dev.type == "cuda":
+            from .rows import select_rows
+            forked = select_rows(tensors, source)
+        else:
+            forked = [t[source] for t in tensors]
+        born = {group: t for (group, _), t in zip(self.GROUPS, forked)}
+        copies = copy_idx.numel()
+        born["xyz"][copies:] += world
+        born["scaling"][copies:] = torch.log(spread / (0.8 * children))
 
+        appended = source.numel()
         total = count + appended
         gone = torch.zeros((total,), dtype=torch.bool, device=dev)
         gone[parent_idx] = True
-        gone |= self.get_opacity.reshape(-1) < min_opacity
+        gone |= torch.sigmoid(torch.cat((self._opacity, born["opacity"]))).reshape(-1) < min_opacity
         if max_screen_size:
-            gone |= self.get_scaling.amax(dim=1) > 0.1 * extent
-            gone |= self.max_radii2D > max_screen_size          # zeros after an append, as in the reference
-        self.prune_points(gone)
+            gone |= torch.exp(torch.cat((self._scaling, born["scaling"]))).amax(dim=1) > 0.1 * extent
+            if not appended:                                    # an append starts the recorded radii again, as in the reference
+                gone |= self.max_radii2D > max_screen_size
+        if not appended:
+            self.prune_points(gone)
+            return
+        self._adopt(self.optimizer.refine(~gone, born))
+        n = self._xyz.shape[0]
+        self.xyz_gradient_accum = torch.zeros((n, 1), device=dev)
+        self.denom = torch.zeros((n, 1), device=dev)
+        self.max_radii2D = torch.zeros((n,), device=dev)
 
     def capture(self):
         """The checkpoint tuple of :61-75, the optimiser's state in torch.optim.Adam's layout."""

@@ -356,10 +356,41 @@ class GaussianAdam:
     def prune(self, keep: torch.Tensor) -> Dict[str, torch.nn.Parameter]:
         """_prune_optimizer (:273-289): keeps the rows selected by the boolean mask ``keep`` of every tensor and
         of both moments; returns the new parameters by group name."""
+        if self._moves_rows_on_the_gpu(keep):
+            return self.refine(keep, None)
         for name, p in self.params.items():
             self.exp_avg[name] = self.exp_avg[name][keep].contiguous()
             self.exp_avg_sq[name] = self.exp_avg_sq[name][keep].contiguous()
             self.params[name] = torch.nn.Parameter(p.detach()[keep].contiguous().requires_grad_(True))
+        return dict(self.params)
+
+    def _moves_rows_on_the_gpu(self, keep: torch.Tensor) -> bool:
+        """Whether ``keep`` and every tensor are what ``compact_rows`` moves: one bool per row, on one GPU."""
+        state = [t for group in (self.params, self.exp_avg, self.exp_avg_sq) for t in group.values()]
+        return (keep.dtype == torch.bool and keep.dim() == 1 and keep.is_cuda
+                and all(t.device == keep.device and t.dim() > 0 and t.shape[0] == keep.shape[0] for t in state))
+
+    @torch.no_grad()
+    def refine(self, keep: torch.Tensor, extension: Optional[Dict[str, torch.Tensor]] = None) -> Dict[str, torch.nn.Parameter]:
+        """``cat_tensors(extension)`` and then ``prune(keep)``, in one pass: ``keep`` has one bool per row, the old
+        ones first and the appended ones behind them.  On the GPU all tensors and moments are moved by one launch and
+        the concatenations are never built (``gsplat_host.rows.compact_rows``)."""
+        if extension is not None and set(extension) != set(self.params):
+            raise ValueError(f"extension must name every tensor: {sorted(self.params)}")
+        if not keep.is_cuda:
+            if extension is not None:
+                self.cat_tensors(extension)
+            return self.prune(keep)
+        from .rows import compact_rows
+        names = list(self.params)
+        more = None
+        if extension is not None:
+            more = [extension[n].detach().to(self.params[n].dtype) for n in names] + [None] * (2 * len(names))
+        rows, _ = compact_rows([self.params[n].detach() for n in names] + [self.exp_avg[n] for n in names]
+                               + [self.exp_avg_sq[n] for n in names], keep, more)
+        for i, n in enumerate(names):
+            self.params[n] = torch.nn.Parameter(rows[i].requires_grad_(True))
+            self.exp_avg[n], self.exp_avg_sq[n] = rows[len(names) + i], rows[2 * len(names) + i]
         return dict(self.params)
 
     @torch.no_grad()

@@ -555,6 +555,32 @@ int gsr_adam_step_clipped(int count, const GsrAdamTensor* h_tensors, const int* 
                           int norm_type, double max_norm, int skip_nonfinite, float* norm,
                           void* scratch, size_t scratch_bytes, void* stream);
 
+/* ---- Rows of many tensors ------------------------------------------------------
+ * What refinement does to the model's six tensors and their two moments each
+ * (scene/gaussian_model.py:258-327, called at :291-403), for any tensors that share their
+ * number of rows.
+ * gsr_keep_rows: index[0 .. *count) (device, room for n) = the positions of the non-zero
+ * bytes of keep (n), ascending; *count (device) their number.  index behind *count is
+ * left as it was.  scratch: gsr_keep_rows_bytes(), 256-byte aligned.
+ * gsr_select_rows: out[j] = row index[j] of `rows` (n_rows of them) followed by
+ * `appended` (n_appended; NULL = rows of zeros), j < n_out, for every tensor of the HOST
+ * array h_tensors.  index: int32 (index_bytes 4) or int64 (8) on the device, in any order
+ * and with repeats; a negative one or one behind the last row gives a row of zeros and
+ * reads nothing.  Rows are contiguous, of row_bytes bytes (below 2^31, 0 allowed), of any
+ * type: they are copied as bytes.  Outputs overlap neither each other nor any input.
+ * At most 2^31 - 2^16 rows on either side. */
+typedef struct GsrRows {
+  const void* rows;
+  const void* appended;
+  void* out;
+  size_t row_bytes;
+} GsrRows;
+size_t gsr_keep_rows_bytes(void);
+int gsr_keep_rows(uint64_t n, const uint8_t* keep, int32_t* index, uint32_t* count, void* scratch,
+                  size_t scratch_bytes, void* stream);
+int gsr_select_rows(int count, const GsrRows* h_tensors, uint64_t n_rows, uint64_t n_appended,
+                    uint64_t n_out, const void* index, int index_bytes, void* stream);
+
 /* ---- Initial scales: mean squared distance to the three nearest neighbours ----
  * distCUDA2 of the reference's second native submodule, simple_knn (call site
  * scene/gaussian_model.py:134, used once, to initialise the scales; the
