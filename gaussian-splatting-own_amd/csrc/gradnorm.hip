@@ -24,20 +24,26 @@ using gsr::kNormBlocks;
 constexpr int kBlock = 512;
 constexpr int kRounds = 4;                                   // 16-byte accesses of a thread in flight
 constexpr uint32_t kChunk = kBlock * kRounds * 16;           // bytes
+constexpr uint32_t kClipBlocks = 1024;                       // workgroups of a clipping launch at most
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 // Tensors are cut into chunks at 16-byte boundaries of the address, so that every access inside is aligned whatever
 // the tensor's own alignment; its first and last vectors may be cut and go element by element.
+struct GradChunk {
+  uintptr_t begin, end;
+  uint32_t first;                                            // number of its first chunk
+  uint32_t type;
+};
+// MOST: a short list is handed over in a short structure (every launch copies its arguments: 3 KB of them cost the
+// host half a microsecond and the kernel's first loads more).
+template <int MOST>
 struct GradChunks {
-  struct One {
-    uintptr_t begin, end;
-    uint32_t first;                                          // number of its first chunk
-    uint32_t type;
-  } t[kGradsPerLaunch];
   uint32_t chunks;
   int count;
+  GradChunk t[MOST];
 };
+constexpr int kFewGrads = 8;
 
 __device__ __forceinline__ float bf16_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
 __device__ __forceinline__ float f16_to_f32(uint32_t h) {
@@ -158,7 +164,8 @@ __device__ __forceinline__ void scale_chunk(float c, uintptr_t base, uintptr_t b
 }
 
 // The tensor that chunk c lies in (the last whose first chunk is not behind it).
-__device__ __forceinline__ int tensor_of(const GradChunks& a, uint32_t c) {
+template <int MOST>
+__device__ __forceinline__ int tensor_of(const GradChunks<MOST>& a, uint32_t c) {
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -167,8 +174,8 @@ __device__ __forceinline__ int tensor_of(const GradChunks& a, uint32_t c) {
   return lo;
 }
 
-template <int NORM>
-__global__ void __launch_bounds__(kBlock) norm_kernel(GradChunks a, double* __restrict__ partials) {
+template <int NORM, int MOST>
+__global__ void __launch_bounds__(kBlock) norm_kernel(GradChunks<MOST> a, double* __restrict__ partials) {
   double acc = 0.0;
   int k = tensor_of(a, blockIdx.x);
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
@@ -198,8 +205,8 @@ __global__ void __launch_bounds__(64) norm_final_kernel(const double* __restrict
 }
 
 // Walks the chunks backwards: what the norm pass read last is still in the last-level cache.
-template <int NORM>
-__global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks a, const double* __restrict__ partials, int used,
+template <int NORM, int MOST>
+__global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks<MOST> a, const double* __restrict__ partials, int used,
                                                       double max_norm, float* __restrict__ norm) {
   const double n = gsr::norm_of_partials<NORM>(partials, used);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
@@ -228,10 +235,11 @@ inline uint64_t chunks_of(const GsrGrad& g) {
 }
 
 // Descriptors of the next launch from h_grads[*at ..), empty tensors left out; advances *at.
-inline void fill(GradChunks& a, int count, const GsrGrad* h_grads, int* at) {
+template <int MOST>
+inline void fill(GradChunks<MOST>& a, int count, const GsrGrad* h_grads, int* at) {
   a.count = 0;
   a.chunks = 0;
-  for (; *at < count && a.count < kGradsPerLaunch; ++*at) {
+  for (; *at < count && a.count < MOST; ++*at) {
     const GsrGrad& g = h_grads[*at];
     const uint64_t chunks = chunks_of(g);
     if (!chunks) continue;
@@ -239,6 +247,50 @@ inline void fill(GradChunks& a, int count, const GsrGrad* h_grads, int* at) {
     a.t[a.count++] = {begin, begin + g.n * size_of(g.type), a.chunks, (uint32_t)g.type};
     a.chunks += (uint32_t)chunks;
   }
+}
+
+template <int MOST>
+int launch_norm(int count, const GsrGrad* h_grads, int norm_type, double* partials, int* used, hipStream_t stream) {
+  uint64_t total = 0;
+  for (int k = 0; k < count; k++) total += chunks_of(h_grads[k]);
+  *used = 0;
+  GradChunks<MOST> a;
+  for (int at = 0; at < count;) {
+    fill(a, count, h_grads, &at);
+    if (!a.chunks) continue;
+    // each launch gets its share of the workgroups, rounded up: at most one more per launch in all
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(a.chunks, ((uint64_t)kNormBlocks * a.chunks + total - 1) / total);
+    double* out = partials + *used;
+    const dim3 grid(blocks), block(kBlock);
+    if (norm_type == GSR_NORM_2) hipLaunchKernelGGL((norm_kernel<GSR_NORM_2, MOST>), grid, block, 0, stream, a, out);
+    else if (norm_type == GSR_NORM_1) hipLaunchKernelGGL((norm_kernel<GSR_NORM_1, MOST>), grid, block, 0, stream, a, out);
+    else hipLaunchKernelGGL((norm_kernel<GSR_NORM_MAX, MOST>), grid, block, 0, stream, a, out);
+    const int rc = gsr::check_launch("grad_norm");
+    if (rc != GSR_OK) return rc;
+    *used += (int)blocks;
+  }
+  return GSR_OK;
+}
+
+template <int MOST>
+int launch_clip(int count, const GsrGrad* h_grads, int norm_type, const double* partials, int used, double max_norm,
+                float* norm, hipStream_t stream) {
+  GradChunks<MOST> a;
+  for (int at = 0; at < count;) {
+    fill(a, count, h_grads, &at);
+    if (!a.chunks) continue;
+    const dim3 grid(std::min<uint32_t>(a.chunks, kClipBlocks)), block(kBlock);
+    if (norm_type == GSR_NORM_2)
+      hipLaunchKernelGGL((clip_kernel<GSR_NORM_2, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm);
+    else if (norm_type == GSR_NORM_1)
+      hipLaunchKernelGGL((clip_kernel<GSR_NORM_1, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm);
+    else
+      hipLaunchKernelGGL((clip_kernel<GSR_NORM_MAX, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm);
+    const int rc = gsr::check_launch("clip_grads");
+    if (rc != GSR_OK) return rc;
+    norm = nullptr;                                          // the first launch has written it
+  }
+  return GSR_OK;
 }
 
 }  // namespace
@@ -271,24 +323,8 @@ int check_norm(const char* what, int count, const GsrGrad* h_grads, int norm_typ
 }
 
 int norm_partials(int count, const GsrGrad* h_grads, int norm_type, double* partials, int* used, hipStream_t stream) {
-  uint64_t total = 0;
-  for (int k = 0; k < count; k++) total += chunks_of(h_grads[k]);
-  *used = 0;
-  GradChunks a;
-  for (int at = 0; at < count;) {
-    fill(a, count, h_grads, &at);
-    if (!a.chunks) continue;
-    // each launch gets its share of the workgroups, rounded up: at most one more per launch in all
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>(a.chunks, ((uint64_t)kNormBlocks * a.chunks + total - 1) / total);
-    double* out = partials + *used;
-    if (norm_type == GSR_NORM_2) hipLaunchKernelGGL(norm_kernel<GSR_NORM_2>, dim3(blocks), dim3(kBlock), 0, stream, a, out);
-    else if (norm_type == GSR_NORM_1) hipLaunchKernelGGL(norm_kernel<GSR_NORM_1>, dim3(blocks), dim3(kBlock), 0, stream, a, out);
-    else hipLaunchKernelGGL(norm_kernel<GSR_NORM_MAX>, dim3(blocks), dim3(kBlock), 0, stream, a, out);
-    const int rc = check_launch("grad_norm");
-    if (rc != GSR_OK) return rc;
-    *used += (int)blocks;
-  }
-  return GSR_OK;
+  if (count <= kFewGrads) return launch_norm<kFewGrads>(count, h_grads, norm_type, partials, used, stream);
+  return launch_norm<kGradsPerLaunch>(count, h_grads, norm_type, partials, used, stream);
 }
 
 }  // namespace gsr
@@ -350,20 +386,7 @@ extern "C" int gsr_clip_grads(int count, const GsrGrad* h_grads, int norm_type, 
   rc = gsr::norm_partials(count, h_grads, norm_type, partials, &used, (hipStream_t)stream);
   if (rc != GSR_OK) return rc;
   if (used == 0) return write_norm(partials, 0, norm_type, norm, (hipStream_t)stream);
-  GradChunks a;
-  for (int at = 0; at < count;) {
-    fill(a, count, h_grads, &at);
-    if (!a.chunks) continue;
-    const uint32_t blocks = std::min<uint32_t>(a.chunks, kNormBlocks * 2);
-    if (norm_type == GSR_NORM_2)
-      hipLaunchKernelGGL(clip_kernel<GSR_NORM_2>, dim3(blocks), dim3(kBlock), 0, (hipStream_t)stream, a, partials, used, max_norm, norm);
-    else if (norm_type == GSR_NORM_1)
-      hipLaunchKernelGGL(clip_kernel<GSR_NORM_1>, dim3(blocks), dim3(kBlock), 0, (hipStream_t)stream, a, partials, used, max_norm, norm);
-    else
-      hipLaunchKernelGGL(clip_kernel<GSR_NORM_MAX>, dim3(blocks), dim3(kBlock), 0, (hipStream_t)stream, a, partials, used, max_norm, norm);
-    rc = gsr::check_launch("clip_grads");
-    if (rc != GSR_OK) return rc;
-    norm = nullptr;                                          // the first launch has written it
-  }
-  return GSR_OK;
+  if (count <= kFewGrads)
+    return launch_clip<kFewGrads>(count, h_grads, norm_type, partials, used, max_norm, norm, (hipStream_t)stream);
+  return launch_clip<kGradsPerLaunch>(count, h_grads, norm_type, partials, used, max_norm, norm, (hipStream_t)stream);
 }

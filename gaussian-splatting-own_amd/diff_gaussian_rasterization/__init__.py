@@ -19,6 +19,7 @@ fails.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import threading
@@ -279,6 +280,20 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _raw_stream(device: int) -> int:
+    """The current stream of GPU ``device`` as a hipStream_t (``torch.cuda.current_stream(device).cuda_stream`` without
+    the stream object around it, which takes 2.7 us to make)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+_stay = contextlib.nullcontext()
+
+
+def _on_device(device: int):
+    """Context in which ``device`` is the current GPU; nothing to do, and nothing done, where it is already."""
+    return _stay if torch.cuda.current_device() == device else torch.cuda.device(device)
 
 
 # Host-side helpers a forward keeps between calls, one set per (host thread, device): two threads that

@@ -13,7 +13,9 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import dataclass
+from itertools import chain
 from typing import Dict, Iterable, List, Optional, Union
 
 import torch
@@ -36,7 +38,7 @@ _lib.gsr_grad_norm_bytes.restype = C.c_size_t
 _lib.gsr_grad_norm_bytes.argtypes = [C.c_int]
 _lib.gsr_grad_norm.argtypes = [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
 _lib.gsr_clip_grads.argtypes = [C.c_int, C.c_void_p, C.c_int, C.c_double, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
-_lib.gsr_adam_step_clipped.argtypes = [C.c_int, C.POINTER(_AdamTensor), C.POINTER(C.c_int), C.c_double, C.c_double, C.c_double,
+_lib.gsr_adam_step_clipped.argtypes = [C.c_int, C.c_void_p, C.c_void_p, C.c_double, C.c_double, C.c_double,
                                        C.c_int, C.c_float, C.c_int, C.c_double, C.c_int, C.c_void_p, C.c_void_p, C.c_size_t,
                                        C.c_void_p]
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}         # GSR_F32, GSR_F16, GSR_BF16 of gsr.h
@@ -213,14 +215,13 @@ def _grad_list(grads: Grads) -> List[torch.Tensor]:
     out = [g for g in grads if g is not None]
     if not out:
         raise ValueError("no gradients given")
-    dev = out[0].device
-    for g in out:
-        if g.dtype not in _TYPES:
-            raise TypeError(f"gradients must be float32, float16 or bfloat16, got {g.dtype}")
-        if not g.is_cuda or g.layout != torch.strided:
-            raise ValueError(f"gradients must be dense tensors on the GPU, got {g.layout} on {g.device}")
-        if g.device != dev:
-            raise ValueError(f"gradients are on {dev} and {g.device}: one call works on one GPU")
+    # the checks of a long list run over it attribute by attribute: a loop over the tensors takes twice as long
+    if not _TYPES.keys() >= {g.dtype for g in out}:
+        raise TypeError(f"gradients must be float32, float16 or bfloat16, got {[g.dtype for g in out if g.dtype not in _TYPES][0]}")
+    if {g.layout for g in out} != {torch.strided} or not all(g.is_cuda for g in out):
+        raise ValueError(f"gradients must be dense tensors on the GPU, got {[(str(g.layout), str(g.device)) for g in out][:8]}")
+    if len({g.get_device() for g in out}) > 1:
+        raise ValueError(f"gradients are on {sorted({str(g.device) for g in out})}: one call works on one GPU")
     return out
 
 
@@ -244,21 +245,18 @@ def _shares_elements(t: torch.Tensor) -> bool:
 
 def _run_norm(what: str, fn, tensors: List[torch.Tensor], code: int, *bound: float) -> torch.Tensor:
     """One norm or clipping call over tensors that fill their memory, on the current stream of their GPU."""
-    dev = tensors[0].device
-    with torch.cuda.device(dev):
-        words: List[int] = []
-        for g in tensors:
-            words += (g.data_ptr(), g.numel(), _TYPES[g.dtype])
-        n = len(tensors)
+    dev, n = tensors[0].device, len(tensors)
+    with _dgr._on_device(dev.index):
+        words = chain.from_iterable(zip([g.data_ptr() for g in tensors], [g.numel() for g in tensors],
+                                        [_TYPES[g.dtype] for g in tensors]))
         nb = _lib.gsr_grad_norm_bytes(n)
         scratch = torch.empty((nb,), dtype=torch.uint8, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        _dgr._run(what, fn, n, (C.c_uint64 * (3 * n))(*words), code, *bound, _dgr._ptr(norm), _dgr._ptr(scratch), nb,
-                  _dgr._stream())
+        _dgr._run(what, fn, n, struct.pack(f"{3 * n}Q", *words), code, *bound, norm.data_ptr(), scratch.data_ptr(), nb,
+                  _dgr._raw_stream(dev.index))
     return norm
 
 
-@torch.no_grad()
 def grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all gradients together, as a float32 scalar on their GPU; nothing waits for it.
 
@@ -266,11 +264,12 @@ def grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
     and bfloat16 mixed as they come, of any shape and strides.  ``norm_type``: 2 (root of the sum of squares), 1 (sum
     of magnitudes) or infinity (the largest magnitude).  Sums are held in 64 bits; a NaN anywhere gives NaN.
     A tensor that is given twice counts twice."""
-    tensors = [g if _fills_its_memory(g) else g.contiguous() for g in _grad_list(grads)]
-    return _run_norm("grad_norm", _lib.gsr_grad_norm, tensors, _norm_code(norm_type))
+    code, tensors = _norm_code(norm_type), _grad_list(grads)
+    if not all(g.is_contiguous() for g in tensors):
+        tensors = [g if _fills_its_memory(g) else g.detach().contiguous() for g in tensors]
+    return _run_norm("grad_norm", _lib.gsr_grad_norm, tensors, code)
 
 
-@torch.no_grad()
 def clip_grads_(grads: Grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """Scales all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` (the rule of
     ``torch.nn.utils.clip_grad_norm_``) and returns the norm they had, a float32 scalar on their GPU.
@@ -283,18 +282,18 @@ def clip_grads_(grads: Grads, max_norm: float, norm_type: float = 2.0) -> torch.
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be at least 0, got {max_norm}")
     code, tensors = _norm_code(norm_type), _grad_list(grads)
-    direct, staged = [], []
-    for g in tensors:
-        if _fills_its_memory(g):
-            direct.append(g)
-        elif _shares_elements(g):
-            raise ValueError(f"a gradient of shape {tuple(g.shape)} and strides {g.stride()} has elements that share memory")
-        else:
-            staged.append((g, g.contiguous()))
-            direct.append(staged[-1][1])
-    norm = _run_norm("clip_grads", _lib.gsr_clip_grads, direct, code, max_norm)
-    for g, scaled in staged:
-        g.copy_(scaled)
+    if all(g.is_contiguous() for g in tensors):
+        norm = _run_norm("clip_grads", _lib.gsr_clip_grads, tensors, code, max_norm)
+    else:
+        # a tensor with gaps between its elements is scaled as a copy without them and copied back
+        staged = [None if _fills_its_memory(g) else g.detach().contiguous() for g in tensors]
+        for g, copy in zip(tensors, staged):
+            if copy is not None and _shares_elements(g):
+                raise ValueError(f"a gradient of shape {tuple(g.shape)} and strides {g.stride()} has elements that share memory")
+        norm = _run_norm("clip_grads", _lib.gsr_clip_grads, [g if c is None else c for g, c in zip(tensors, staged)], code, max_norm)
+        for g, copy in zip(tensors, staged):
+            if copy is not None:
+                g.detach().copy_(copy)
     torch.autograd.graph.increment_version(tensors)          # written behind autograd's back
     return norm
 
@@ -473,43 +472,46 @@ class GaussianAdam:
             max_norm, code = float(max_norm), _norm_code(norm_type)
             if not max_norm >= 0.0:
                 raise ValueError(f"max_norm must be at least 0, got {max_norm}")
-        arr, types = (_AdamTensor * MAX_TENSORS)(), (C.c_int * MAX_TENSORS)()
-        n = 0
-        dev = next(iter(self.params.values())).device if self.params else torch.device("cuda")
+        rows: List[tuple] = []                     # the fields of a GsrAdamTensor each
+        types: List[int] = []
+        dev = next(iter(self.params.values())).device if self.params else torch.device("cuda", torch.cuda.current_device())
         keep: List[torch.Tensor] = []
         for name, p in self.params.items():
             g = grads[name] if grads is not None else p.grad
             if g is None:
                 continue
-            if g.numel() != p.numel():
-                raise ValueError(f"{name}: gradient has {g.numel()} elements, parameter {p.numel()}")
-            if g.numel() == 0:
+            n = p.numel()
+            if g.numel() != n:
+                raise ValueError(f"{name}: gradient has {g.numel()} elements, parameter {n}")
+            if n == 0:
                 continue
             if max_norm is None:
                 g = _dgr._f32(g, f"grad of {name}")
             else:
-                if g.dtype not in _TYPES:
+                kind = _TYPES.get(g.dtype)
+                if kind is None:
                     raise TypeError(f"grad of {name} must be float32, float16 or bfloat16, got {g.dtype}")
                 if g.device != dev or p.device != dev:
                     raise ValueError(f"{name}: parameter and gradient must be on {dev}, they are on {p.device} and {g.device}")
-                types[n] = _TYPES[g.dtype]
+                types.append(kind)
                 g = g.contiguous()
             keep.append(g)
-            arr[n] = _AdamTensor(p.data_ptr(), g.data_ptr(), self.exp_avg[name].data_ptr(),
-                                 self.exp_avg_sq[name].data_ptr(), p.numel(), float(self.lrs[name]), 0)
-            n += 1
+            rows.append((p.data_ptr(), g.data_ptr(), self.exp_avg[name].data_ptr(), self.exp_avg_sq[name].data_ptr(), n,
+                         float(self.lrs[name]), 0))
         self.step_count += 1
         if max_norm is None:
-            _dgr._run("adam_step", _lib.gsr_adam_step, n, arr, float(self.betas[0]), float(self.betas[1]),
-                      float(self.eps), int(self.step_count), float(grad_scale), _dgr._stream())
+            _dgr._run("adam_step", _lib.gsr_adam_step, len(rows), (_AdamTensor * MAX_TENSORS)(*rows), float(self.betas[0]),
+                      float(self.betas[1]), float(self.eps), int(self.step_count), float(grad_scale), _dgr._stream())
             return None
-        with torch.cuda.device(dev):
-            nb = _lib.gsr_grad_norm_bytes(n)
+        with _dgr._on_device(dev.index):
+            count = len(rows)
+            nb = _lib.gsr_grad_norm_bytes(count)
             scratch = torch.empty((nb,), dtype=torch.uint8, device=dev)
             norm = torch.empty((), dtype=torch.float32, device=dev)
-            _dgr._run("adam_step", _lib.gsr_adam_step_clipped, n, arr, types, float(self.betas[0]), float(self.betas[1]),
-                      float(self.eps), int(self.step_count), float(grad_scale), code, max_norm, int(bool(skip_nonfinite)),
-                      _dgr._ptr(norm), _dgr._ptr(scratch), nb, _dgr._stream())
+            _dgr._run("adam_step", _lib.gsr_adam_step_clipped, count, struct.pack("5Qfi" * count, *chain.from_iterable(rows)),
+                      struct.pack(f"{count}i", *types), float(self.betas[0]), float(self.betas[1]), float(self.eps),
+                      int(self.step_count), float(grad_scale), code, max_norm, int(bool(skip_nonfinite)), norm.data_ptr(),
+                      scratch.data_ptr(), nb, _dgr._raw_stream(dev.index))
         return norm
 
     def zero_grad(self, set_to_none: bool = True) -> None:

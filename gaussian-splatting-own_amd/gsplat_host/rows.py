@@ -9,6 +9,9 @@ through these copies: they change what an optimiser works on, between its steps.
 from __future__ import annotations
 
 import ctypes as C
+import itertools
+import struct
+from itertools import chain
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -18,7 +21,7 @@ import diff_gaussian_rasterization as _dgr
 _lib = _dgr._lib
 _lib.gsr_keep_rows_bytes.restype = C.c_size_t
 _lib.gsr_keep_rows_bytes.argtypes = []
-_lib.gsr_keep_rows.argtypes = [C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+_lib.gsr_keep_rows.argtypes = [C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_size_t, C.c_void_p]
 _lib.gsr_select_rows.argtypes = [C.c_int, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_int, C.c_void_p]
 MAX_ROWS = 0x7FFF0000                  # row numbers are 32-bit
 
@@ -27,38 +30,37 @@ def _checked(tensors: Sequence[torch.Tensor]) -> Tuple[List[torch.Tensor], torch
     tensors = list(tensors)
     if not tensors:
         raise ValueError("no tensors given")
-    dev, rows = tensors[0].device, tensors[0].shape[0] if tensors[0].dim() else -1
-    for t in tensors:
-        if not t.is_cuda or t.layout != torch.strided:
-            raise ValueError(f"rows are moved between dense tensors on the GPU, got {t.layout} on {t.device}")
-        if t.device != dev:
-            raise ValueError(f"tensors are on {dev} and {t.device}: one call works on one GPU")
-        if t.dim() == 0 or t.shape[0] != rows:
-            raise ValueError(f"tensors must share their first dimension, got shapes {[tuple(x.shape) for x in tensors]}")
+    if {t.layout for t in tensors} != {torch.strided} or not all(t.is_cuda for t in tensors):
+        raise ValueError("rows are moved between dense tensors on the GPU, got "
+                         f"{[(str(t.layout), str(t.device)) for t in tensors][:8]}")
+    if len({t.get_device() for t in tensors}) > 1:
+        raise ValueError(f"tensors are on {sorted({str(t.device) for t in tensors})}: one call works on one GPU")
+    shapes = [t.shape for t in tensors]
+    rows = {s[0] if s else -1 for s in shapes}
+    if len(rows) > 1 or -1 in rows:
+        raise ValueError(f"tensors must share their first dimension, got shapes {[tuple(s) for s in shapes]}")
+    rows = rows.pop()
     if rows > MAX_ROWS:
         raise ValueError(f"{rows} rows: at most {MAX_ROWS}")
-    return tensors, dev, rows
+    return tensors, tensors[0].device, rows
 
 
 def _move(tensors: List[torch.Tensor], appended: List[Optional[torch.Tensor]], rows: int, extra: int, index: torch.Tensor,
           count: int) -> List[torch.Tensor]:
-    out, words, hold = [], [], []
-    for t, e in zip(tensors, appended):
-        o = torch.empty((count,) + t.shape[1:], dtype=t.dtype, device=t.device)
-        t = t.contiguous()
-        e = None if e is None else e.contiguous()
-        hold.append((t, e))
-        out.append(o)
-        row = t.element_size()
-        for s in t.shape[1:]:
-            row *= s
-        words += (t.data_ptr(), 0 if e is None else e.data_ptr(), o.data_ptr(), row)
-    _dgr._run("select_rows", _lib.gsr_select_rows, len(out), (C.c_uint64 * len(words))(*words), rows, extra, count,
-              _dgr._ptr(index), index.element_size(), _dgr._stream())
+    out = [t.new_empty((count, *t.shape[1:])) for t in tensors]
+    if count:
+        words = chain.from_iterable(
+            (t.data_ptr(), 0 if e is None else e.data_ptr(), o.data_ptr(), o.numel() // count * o.element_size())
+            for t, e, o in zip(tensors, appended, out))
+        _dgr._run("select_rows", _lib.gsr_select_rows, len(out), struct.pack(f"{4 * len(out)}Q", *words), rows, extra, count,
+                  index.data_ptr(), index.element_size(), _dgr._raw_stream(index.get_device()))
     return out
 
 
-@torch.no_grad()
+def _contiguous(tensors: Sequence[Optional[torch.Tensor]]) -> List[Optional[torch.Tensor]]:
+    return [None if t is None else t.detach().contiguous() for t in tensors]
+
+
 def select_rows(tensors: Sequence[torch.Tensor], index: torch.Tensor) -> List[torch.Tensor]:
     """``[t[index] for t in tensors]`` in one launch: new tensors whose row j is row ``index[j]`` of the old ones.
 
@@ -69,13 +71,39 @@ def select_rows(tensors: Sequence[torch.Tensor], index: torch.Tensor) -> List[to
         raise TypeError(f"index must be a one-dimensional int32 or int64 tensor, got {index.dtype} of shape {tuple(index.shape)}")
     if index.device != dev:
         raise ValueError(f"index is on {index.device}, the tensors are on {dev}")
-    if index.numel() > MAX_ROWS:
-        raise ValueError(f"{index.numel()} rows: at most {MAX_ROWS}")
-    with torch.cuda.device(dev):
-        return _move(tensors, [None] * len(tensors), rows, 0, index.contiguous(), index.numel())
+    count = index.numel()
+    if count > MAX_ROWS:
+        raise ValueError(f"{count} rows: at most {MAX_ROWS}")
+    with _dgr._on_device(dev.index):
+        return _move(_contiguous(tensors), [None] * len(tensors), rows, 0, index.contiguous(), count)
 
 
-@torch.no_grad()
+_tickets = itertools.count(1)
+
+
+def _landing(dev: torch.device):
+    """This thread's pinned word for ``dev`` that a count of kept rows lands in: (the tensor that owns it, the word)."""
+    slots = _dgr._per_device(dev)
+    if "kept_rows" not in slots:
+        word = torch.zeros((1,), dtype=torch.int64, pin_memory=True)
+        slots["kept_rows"] = word, C.c_uint64.from_address(word.data_ptr())
+    return slots["kept_rows"]
+
+
+def _await_count(word: C.c_uint64, ticket: int, dev: torch.device) -> int:
+    """The count that lands in ``word`` with ``ticket``.  Looks for it for a millisecond or two, which saves the wait
+    for a copy to the host (13 us); a stream with more work than that before it is waited for."""
+    for _ in range(10_000):
+        value = word.value
+        if value >> 32 == ticket:
+            return value & 0xFFFFFFFF
+    torch.cuda.current_stream(dev).synchronize()
+    value = word.value
+    if value >> 32 != ticket:
+        raise RuntimeError("libgsr_hip keep_rows failed: the number of kept rows never arrived")
+    return value & 0xFFFFFFFF
+
+
 def compact_rows(tensors: Sequence[torch.Tensor], keep: torch.Tensor,
                  appended: Optional[Sequence[Optional[torch.Tensor]]] = None) -> Tuple[List[torch.Tensor], torch.Tensor]:
     """``([torch.cat((t, a))[keep] for t, a in zip(tensors, appended)], index)`` without the concatenations.
@@ -83,7 +111,8 @@ def compact_rows(tensors: Sequence[torch.Tensor], keep: torch.Tensor,
     ``keep``: one bool per row, first the tensors' rows, then the appended ones.  ``appended``: for each tensor the rows
     behind its own, or None for rows of zeros (the moments of new Gaussians); None altogether: nothing is appended.
     ``index`` (int32): the positions of the kept rows, so ``index[j]`` is where row j of the results came from.
-    The order stays.  The number of kept rows sizes the results, so the call waits for the GPU once."""
+    The order stays.  The number of kept rows sizes the results, so the host waits for it and the call cannot be
+    captured into a graph."""
     tensors, dev, rows = _checked(tensors)
     if keep.dtype != torch.bool or keep.dim() != 1:
         raise TypeError(f"keep must be a one-dimensional bool tensor, got {keep.dtype} of shape {tuple(keep.shape)}")
@@ -97,16 +126,21 @@ def compact_rows(tensors: Sequence[torch.Tensor], keep: torch.Tensor,
     if len(more) != len(tensors):
         raise ValueError(f"{len(more)} appended entries for {len(tensors)} tensors")
     for t, e in zip(tensors, more):
-        if e is not None and (e.shape != (extra,) + t.shape[1:] or e.dtype != t.dtype or e.device != dev or e.layout != torch.strided):
+        if e is not None and (e.shape != (extra, *t.shape[1:]) or e.dtype != t.dtype or e.device != dev or e.layout != torch.strided):
             raise ValueError(f"appended rows of shape {tuple(e.shape)}, {e.dtype} on {e.device} do not fit {extra} rows of a "
                              f"tensor of shape {tuple(t.shape)}, {t.dtype} on {dev}")
-    with torch.cuda.device(dev):
+    with _dgr._on_device(dev.index):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("compact_rows reads the number of kept rows and cannot be captured into a graph; select_rows can")
         keep = keep.contiguous()
         nb = _lib.gsr_keep_rows_bytes()
         scratch = torch.empty((nb,), dtype=torch.uint8, device=dev)
-        index = torch.empty((total + 1,), dtype=torch.int32, device=dev)          # and the count behind them
-        _dgr._run("keep_rows", _lib.gsr_keep_rows, total, _dgr._ptr(keep), _dgr._ptr(index),
-                  C.c_void_p(index.data_ptr() + 4 * total), _dgr._ptr(scratch), nb, _dgr._stream())
-        count = int(index[total])
+        index = torch.empty((total,), dtype=torch.int32, device=dev)
+        _, word = _landing(dev)
+        ticket = next(_tickets) & 0xFFFFFFFF or next(_tickets) & 0xFFFFFFFF       # never 0
+        _dgr._run("keep_rows", _lib.gsr_keep_rows, total, keep.data_ptr(), index.data_ptr(), C.addressof(word), ticket,
+                  scratch.data_ptr(), nb, _dgr._raw_stream(dev.index))
+        tensors, more = _contiguous(tensors), _contiguous(more)                   # while the GPU counts
+        count = _await_count(word, ticket, dev)
         index = index[:count]
         return _move(tensors, more, rows, extra, index, count), index

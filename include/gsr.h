@@ -559,9 +559,12 @@ int gsr_adam_step_clipped(int count, const GsrAdamTensor* h_tensors, const int* 
  * What refinement does to the model's six tensors and their two moments each
  * (scene/gaussian_model.py:258-327, called at :291-403), for any tensors that share their
  * number of rows.
- * gsr_keep_rows: index[0 .. *count) (device, room for n) = the positions of the non-zero
- * bytes of keep (n), ascending; *count (device) their number.  index behind *count is
- * left as it was.  scratch: gsr_keep_rows_bytes(), 256-byte aligned.
+ * gsr_keep_rows: index[0 .. count) (device, room for n) = the positions of the non-zero
+ * bytes of keep (n), ascending; what lies behind is left as it was.  *landing = count |
+ * ticket << 32, one 64-bit store: device memory, or pinned host memory at the address
+ * the device has for it, where the host can wait for a ticket it has not used before
+ * instead of for the stream (index is complete for what the stream runs next).
+ * scratch: gsr_keep_rows_bytes(), 256-byte aligned.
  * gsr_select_rows: out[j] = row index[j] of `rows` (n_rows of them) followed by
  * `appended` (n_appended; NULL = rows of zeros), j < n_out, for every tensor of the HOST
  * array h_tensors.  index: int32 (index_bytes 4) or int64 (8) on the device, in any order
@@ -576,8 +579,8 @@ typedef struct GsrRows {
   size_t row_bytes;
 } GsrRows;
 size_t gsr_keep_rows_bytes(void);
-int gsr_keep_rows(uint64_t n, const uint8_t* keep, int32_t* index, uint32_t* count, void* scratch,
-                  size_t scratch_bytes, void* stream);
+int gsr_keep_rows(uint64_t n, const uint8_t* keep, int32_t* index, uint64_t* landing, uint32_t ticket,
+                  void* scratch, size_t scratch_bytes, void* stream);
 int gsr_select_rows(int count, const GsrRows* h_tensors, uint64_t n_rows, uint64_t n_appended,
                     uint64_t n_out, const void* index, int index_bytes, void* stream);
 

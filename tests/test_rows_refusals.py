@@ -39,14 +39,15 @@ def test_select_checks():
 def test_keep_checks():
     nb = lib.gsr_keep_rows_bytes()
     assert nb % 256 == 0
-    assert lib.gsr_keep_rows(1 << 31, FAKE, FAKE, FAKE, FAKE, nb, None) == -1 and "rows" in last()
+    assert lib.gsr_keep_rows(1 << 31, FAKE, FAKE, FAKE, 1, FAKE, nb, None) == -1 and "rows" in last()
     for hole in range(3):
         ptrs = [FAKE, FAKE, FAKE]
         ptrs[hole] = None
-        assert lib.gsr_keep_rows(10, *ptrs, FAKE, nb, None) == -1 and "null" in last()
-    assert lib.gsr_keep_rows(10, FAKE, FAKE, FAKE, FAKE, nb - 1, None) == -3
-    assert lib.gsr_keep_rows(10, FAKE, FAKE, FAKE, FAKE + 4, nb, None) == -3
-    assert lib.gsr_keep_rows(10, FAKE, FAKE, FAKE, None, nb, None) == -3
+        assert lib.gsr_keep_rows(10, *ptrs, 1, FAKE, nb, None) == -1 and "null" in last()
+    assert lib.gsr_keep_rows(10, FAKE, FAKE, FAKE + 4, 1, FAKE, nb, None) == -1 and "aligned" in last()
+    assert lib.gsr_keep_rows(10, FAKE, FAKE, FAKE, 1, FAKE, nb - 1, None) == -3
+    assert lib.gsr_keep_rows(10, FAKE, FAKE, FAKE, 1, FAKE + 4, nb, None) == -3
+    assert lib.gsr_keep_rows(10, FAKE, FAKE, FAKE, 1, None, nb, None) == -3
 
 
 def test_python_checks():
