@@ -5,16 +5,18 @@
 
 namespace gsr {
 
-// Workgroups of one norm pass over all its launches, and so the partial results that every clipping wave joins again
-// (four or eight a lane).
+// Workgroups of a launch of the norm pass at most, and so its partial results.
 constexpr int kNormBlocks = 512;
+// Partial results that every clipping wave joins by itself; more of them (over 480 tensors) are joined by a kernel of
+// their own first, which costs a launch (4 us) but not their reading by every wave.
+constexpr int kMostJoined = 4 * kNormBlocks;
 // Descriptors that fit one launch's kernel arguments (4 KB).
 constexpr int kGradsPerLaunch = 120;
 
 // Writes the partial results of all gradients to `partials` (norm_partials_most(count) doubles) and their number to
-// *used (0 when there is no element).  Arguments have been checked.
+// *used (0 when there is no element, at most kMostJoined).  Arguments have been checked.
 int norm_partials(int count, const GsrGrad* h_grads, int norm_type, double* partials, int* used, hipStream_t stream);
-inline int norm_partials_most(int count) { return kNormBlocks + (count + kGradsPerLaunch - 1) / kGradsPerLaunch; }
+inline size_t norm_partials_most(int count) { return kNormBlocks * ((size_t)count / kGradsPerLaunch + 1); }
 // GSR_OK if the list, the norm's type and the scratch are usable; the message names `what`.
 int check_norm(const char* what, int count, const GsrGrad* h_grads, int norm_type, const float* norm, const void* scratch,
                size_t scratch_bytes);

@@ -174,6 +174,19 @@ __device__ __forceinline__ int tensor_of(const GradChunks<MOST>& a, uint32_t c) 
   return lo;
 }
 
+// Joins the workgroup's results into *out.
+template <int NORM>
+__device__ __forceinline__ void join_block(double acc, double* out) {
+  __shared__ double s_wave[kBlock / 64];
+  acc = gsr::norm_join_wave<NORM>(acc);
+  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kBlock / 64; w++) acc = gsr::norm_join<NORM>(acc, s_wave[w]);
+    *out = acc;
+  }
+}
+
 template <int NORM, int MOST>
 __global__ void __launch_bounds__(kBlock) norm_kernel(GradChunks<MOST> a, double* __restrict__ partials) {
   double acc = 0.0;
@@ -188,14 +201,15 @@ __global__ void __launch_bounds__(kBlock) norm_kernel(GradChunks<MOST> a, double
       default: acc = add_chunk<NORM, GSR_BF16>(acc, base, begin, end); break;
     }
   }
-  __shared__ double s_wave[kBlock / 64];
-  acc = gsr::norm_join_wave<NORM>(acc);
-  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = acc;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kBlock / 64; w++) acc = gsr::norm_join<NORM>(acc, s_wave[w]);
-    partials[blockIdx.x] = acc;
-  }
+  join_block<NORM>(acc, partials + blockIdx.x);
+}
+
+// The partial results of very many launches, joined to one in front of the kernels that take them.
+template <int NORM>
+__global__ void __launch_bounds__(kBlock) norm_join_kernel(double* __restrict__ partials, int used) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < used; i += kBlock) acc = gsr::norm_join<NORM>(acc, partials[i]);
+  join_block<NORM>(acc, partials);                           // behind a barrier: every thread has read its share
 }
 
 template <int NORM>
@@ -251,23 +265,18 @@ inline void fill(GradChunks<MOST>& a, int count, const GsrGrad* h_grads, int* at
 
 template <int MOST>
 int launch_norm(int count, const GsrGrad* h_grads, int norm_type, double* partials, int* used, hipStream_t stream) {
-  uint64_t total = 0;
-  for (int k = 0; k < count; k++) total += chunks_of(h_grads[k]);
-  *used = 0;
   GradChunks<MOST> a;
   for (int at = 0; at < count;) {
     fill(a, count, h_grads, &at);
     if (!a.chunks) continue;
-    // each launch gets its share of the workgroups, rounded up: at most one more per launch in all
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>(a.chunks, ((uint64_t)kNormBlocks * a.chunks + total - 1) / total);
     double* out = partials + *used;
-    const dim3 grid(blocks), block(kBlock);
+    const dim3 grid(std::min<uint32_t>(a.chunks, kNormBlocks)), block(kBlock);
     if (norm_type == GSR_NORM_2) hipLaunchKernelGGL((norm_kernel<GSR_NORM_2, MOST>), grid, block, 0, stream, a, out);
     else if (norm_type == GSR_NORM_1) hipLaunchKernelGGL((norm_kernel<GSR_NORM_1, MOST>), grid, block, 0, stream, a, out);
     else hipLaunchKernelGGL((norm_kernel<GSR_NORM_MAX, MOST>), grid, block, 0, stream, a, out);
     const int rc = gsr::check_launch("grad_norm");
     if (rc != GSR_OK) return rc;
-    *used += (int)blocks;
+    *used += (int)grid.x;
   }
   return GSR_OK;
 }
@@ -323,8 +332,15 @@ int check_norm(const char* what, int count, const GsrGrad* h_grads, int norm_typ
 }
 
 int norm_partials(int count, const GsrGrad* h_grads, int norm_type, double* partials, int* used, hipStream_t stream) {
-  if (count <= kFewGrads) return launch_norm<kFewGrads>(count, h_grads, norm_type, partials, used, stream);
-  return launch_norm<kGradsPerLaunch>(count, h_grads, norm_type, partials, used, stream);
+  *used = 0;
+  const int rc = count <= kFewGrads ? launch_norm<kFewGrads>(count, h_grads, norm_type, partials, used, stream)
+                                    : launch_norm<kGradsPerLaunch>(count, h_grads, norm_type, partials, used, stream);
+  if (rc != GSR_OK || *used <= kMostJoined) return rc;
+  if (norm_type == GSR_NORM_2) hipLaunchKernelGGL(norm_join_kernel<GSR_NORM_2>, dim3(1), dim3(kBlock), 0, stream, partials, *used);
+  else if (norm_type == GSR_NORM_1) hipLaunchKernelGGL(norm_join_kernel<GSR_NORM_1>, dim3(1), dim3(kBlock), 0, stream, partials, *used);
+  else hipLaunchKernelGGL(norm_join_kernel<GSR_NORM_MAX>, dim3(1), dim3(kBlock), 0, stream, partials, *used);
+  *used = 1;
+  return check_launch("grad_norm");
 }
 
 }  // namespace gsr

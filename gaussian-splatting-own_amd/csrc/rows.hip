@@ -165,6 +165,9 @@ __global__ void __launch_bounds__(kBlock) move_kernel(Moves a) {
 constexpr int kTile = kBlock * 16;                 // flags a workgroup takes at a time
 constexpr uint32_t kMostBlocks = 1024;             // every workgroup adds up the counts of those before it
 
+// Up to here one workgroup takes all tiles and no counts are needed: a launch (3.5 us for the host) against 0.6 us a tile.
+constexpr uint32_t kFewTiles = 4;
+
 struct Flags {
   uintptr_t base;                                  // keep, rounded down to 16 bytes
   uint32_t skip;                                   // bytes of that which are not flags
@@ -268,7 +271,7 @@ extern "C" int gsr_keep_rows(uint64_t n, const uint8_t* keep, int32_t* index, ui
   f.end = f.skip + (uint32_t)n;
   f.tiles = (f.end + kTile - 1) / kTile;
   if (n == 0) f.tiles = 0;
-  f.tiles_per_block = std::max(1u, (f.tiles + kMostBlocks - 1) / kMostBlocks);
+  f.tiles_per_block = f.tiles <= kFewTiles ? std::max(1u, f.tiles) : (f.tiles + kMostBlocks - 1) / kMostBlocks;
   const uint32_t blocks = std::max(1u, (f.tiles + f.tiles_per_block - 1) / f.tiles_per_block);
   uint32_t* counts = (uint32_t*)scratch;
   if (blocks > 1) {                                // one workgroup has nothing before it

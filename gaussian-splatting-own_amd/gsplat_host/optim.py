@@ -216,12 +216,14 @@ def _grad_list(grads: Grads) -> List[torch.Tensor]:
     if not out:
         raise ValueError("no gradients given")
     # the checks of a long list run over it attribute by attribute: a loop over the tensors takes twice as long
-    if not _TYPES.keys() >= {g.dtype for g in out}:
-        raise TypeError(f"gradients must be float32, float16 or bfloat16, got {[g.dtype for g in out if g.dtype not in _TYPES][0]}")
-    if {g.layout for g in out} != {torch.strided} or not all(g.is_cuda for g in out):
+    dtypes = {g.dtype for g in out}
+    if not _TYPES.keys() >= dtypes:
+        raise TypeError(f"gradients must be float32, float16 or bfloat16, got {sorted(map(str, dtypes - _TYPES.keys()))}")
+    devices = {g.get_device() for g in out}
+    if -1 in devices or {g.layout for g in out} != {torch.strided}:
         raise ValueError(f"gradients must be dense tensors on the GPU, got {[(str(g.layout), str(g.device)) for g in out][:8]}")
-    if len({g.get_device() for g in out}) > 1:
-        raise ValueError(f"gradients are on {sorted({str(g.device) for g in out})}: one call works on one GPU")
+    if len(devices) > 1:
+        raise ValueError(f"gradients are on GPUs {sorted(devices)}: one call works on one GPU")
     return out
 
 

@@ -10,8 +10,8 @@ from __future__ import annotations
 
 import ctypes as C
 import itertools
+import math
 import struct
-from itertools import chain
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -45,20 +45,27 @@ def _checked(tensors: Sequence[torch.Tensor]) -> Tuple[List[torch.Tensor], torch
     return tensors, tensors[0].device, rows
 
 
-def _move(tensors: List[torch.Tensor], appended: List[Optional[torch.Tensor]], rows: int, extra: int, index: torch.Tensor,
-          count: int) -> List[torch.Tensor]:
-    out = [t.new_empty((count, *t.shape[1:])) for t in tensors]
-    if count:
-        words = chain.from_iterable(
-            (t.data_ptr(), 0 if e is None else e.data_ptr(), o.data_ptr(), o.numel() // count * o.element_size())
-            for t, e, o in zip(tensors, appended, out))
-        _dgr._run("select_rows", _lib.gsr_select_rows, len(out), struct.pack(f"{4 * len(out)}Q", *words), rows, extra, count,
-                  index.data_ptr(), index.element_size(), _dgr._raw_stream(index.get_device()))
-    return out
-
-
 def _contiguous(tensors: Sequence[Optional[torch.Tensor]]) -> List[Optional[torch.Tensor]]:
-    return [None if t is None else t.detach().contiguous() for t in tensors]
+    return [t if t is None or t.is_contiguous() else t.detach().contiguous() for t in tensors]
+
+
+class _Move:
+    """A move of rows, as far as it can be prepared before the number of rows is known; ``to`` launches it."""
+
+    def __init__(self, tensors: List[torch.Tensor], appended: List[Optional[torch.Tensor]], rows: int, extra: int):
+        self.tensors, self.appended = _contiguous(tensors), _contiguous(appended)     # kept alive until the launch
+        self.tails = [t.shape[1:] for t in self.tensors]
+        self.fixed = [(t.data_ptr(), 0 if e is None else e.data_ptr(), math.prod(s) * t.element_size())
+                      for t, e, s in zip(self.tensors, self.appended, self.tails)]
+        self.rows, self.extra = rows, extra
+
+    def to(self, index: torch.Tensor, count: int) -> List[torch.Tensor]:
+        out = [t.new_empty((count, *s)) for t, s in zip(self.tensors, self.tails)]
+        if count:
+            words = [w for (t, e, row), o in zip(self.fixed, out) for w in (t, e, o.data_ptr(), row)]
+            _dgr._run("select_rows", _lib.gsr_select_rows, len(out), struct.pack(f"{len(words)}Q", *words), self.rows,
+                      self.extra, count, index.data_ptr(), index.element_size(), _dgr._raw_stream(index.get_device()))
+        return out
 
 
 def select_rows(tensors: Sequence[torch.Tensor], index: torch.Tensor) -> List[torch.Tensor]:
@@ -75,7 +82,7 @@ def select_rows(tensors: Sequence[torch.Tensor], index: torch.Tensor) -> List[to
     if count > MAX_ROWS:
         raise ValueError(f"{count} rows: at most {MAX_ROWS}")
     with _dgr._on_device(dev.index):
-        return _move(_contiguous(tensors), [None] * len(tensors), rows, 0, index.contiguous(), count)
+        return _Move(tensors, [None] * len(tensors), rows, 0).to(index.contiguous(), count)
 
 
 _tickets = itertools.count(1)
@@ -140,7 +147,7 @@ def compact_rows(tensors: Sequence[torch.Tensor], keep: torch.Tensor,
         ticket = next(_tickets) & 0xFFFFFFFF or next(_tickets) & 0xFFFFFFFF       # never 0
         _dgr._run("keep_rows", _lib.gsr_keep_rows, total, keep.data_ptr(), index.data_ptr(), C.addressof(word), ticket,
                   scratch.data_ptr(), nb, _dgr._raw_stream(dev.index))
-        tensors, more = _contiguous(tensors), _contiguous(more)                   # while the GPU counts
+        move = _Move(tensors, more, rows, extra)                                  # while the GPU counts
         count = _await_count(word, ticket, dev)
         index = index[:count]
-        return _move(tensors, more, rows, extra, index, count), index
+        return move.to(index, count), index

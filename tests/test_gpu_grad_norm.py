@@ -419,3 +419,16 @@ def test_training_with_clipping_end_to_end():
         # the same factor on the same gradients, once inside the step: the same bits
         assert torch.equal(clone[k], opt.params[k].detach()) and torch.equal(other.exp_avg[k], opt.exp_avg[k])
     assert float(arena.norm()) <= norm / 7 * (1 + 1e-5)
+
+
+def test_lists_whose_partial_results_are_joined_first():
+    """601 tensors of several chunks each: more partial results than a clipping wave joins by itself."""
+    from gsplat_host.optim import clip_grads_, grad_norm
+    pool = values(601 * 81_921, torch.bfloat16, 3)
+    tensors = list(pool.split(81_921))
+    before = pool.clone()
+    for p in NORMS:
+        check_norm(grad_norm(tensors, p), [before], p)
+    bound = 0.2 * norm64([before], 2.0)
+    check_norm(clip_grads_(tensors, bound), [before], 2.0)
+    check_clipped(pool, before, factor64(norm64([before], 2.0), bound))
