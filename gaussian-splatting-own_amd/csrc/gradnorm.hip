@@ -103,26 +103,25 @@ __device__ __forceinline__ double add_vector(double acc, u4 v) {
   return add_word<NORM, TYPE>(acc, v.w);
 }
 
+// A thread's vectors of the chunk at `base`: all that lie wholly inside the tensor are requested before the first is
+// used; the one or two of a tensor that its ends cut go element by element behind them.
 template <int NORM, int TYPE>
 __device__ __forceinline__ double add_chunk(double acc, uintptr_t base, uintptr_t begin, uintptr_t end) {
   const uintptr_t mine = base + threadIdx.x * 16u;
-  if (base >= begin && base + kChunk <= end) {
-    u4 v[kRounds];
+  u4 v[kRounds];
 #pragma unroll
-    for (int r = 0; r < kRounds; r++) v[r] = *(const u4*)(mine + (uintptr_t)r * kBlock * 16);
-#pragma unroll
-    for (int r = 0; r < kRounds; r++) acc = add_vector<NORM, TYPE>(acc, v[r]);
-    return acc;
-  }
   for (int r = 0; r < kRounds; r++) {
     const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
-    if (a >= end) break;
-    if (a >= begin && a + 16 <= end) {
-      acc = add_vector<NORM, TYPE>(acc, *(const u4*)a);
-    } else {
+    v[r] = a >= begin && a + 16 <= end ? *(const u4*)a : (u4){0, 0, 0, 0};     // zeros add nothing
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; r++) acc = add_vector<NORM, TYPE>(acc, v[r]);
+  if (base >= begin && base + kChunk <= end) return acc;
+  for (int r = 0; r < kRounds; r++) {
+    const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
+    if (a < end && (a < begin || a + 16 > end))
       for (uintptr_t e = a < begin ? begin : a; e < a + 16 && e < end; e += Elem<TYPE>::kSize)
         acc = add<NORM>(acc, Elem<TYPE>::load(e));
-    }
   }
   return acc;
 }
@@ -143,33 +142,42 @@ __device__ __forceinline__ u4 scale_vector(u4 v, float c) {
 template <int TYPE>
 __device__ __forceinline__ void scale_chunk(float c, uintptr_t base, uintptr_t begin, uintptr_t end) {
   const uintptr_t mine = base + threadIdx.x * 16u;
-  if (base >= begin && base + kChunk <= end) {
-    u4 v[kRounds];
+  u4 v[kRounds];
 #pragma unroll
-    for (int r = 0; r < kRounds; r++) v[r] = *(const u4*)(mine + (uintptr_t)r * kBlock * 16);
-#pragma unroll
-    for (int r = 0; r < kRounds; r++) *(u4*)(mine + (uintptr_t)r * kBlock * 16) = scale_vector<TYPE>(v[r], c);
-    return;
-  }
   for (int r = 0; r < kRounds; r++) {
     const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
-    if (a >= end) break;
-    if (a >= begin && a + 16 <= end) {
-      *(u4*)a = scale_vector<TYPE>(*(const u4*)a, c);
-    } else {
+    v[r] = a >= begin && a + 16 <= end ? *(const u4*)a : (u4){0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; r++) {
+    const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
+    if (a >= begin && a + 16 <= end) *(u4*)a = scale_vector<TYPE>(v[r], c);
+  }
+  if (base >= begin && base + kChunk <= end) return;
+  for (int r = 0; r < kRounds; r++) {
+    const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
+    if (a < end && (a < begin || a + 16 > end))
       for (uintptr_t e = a < begin ? begin : a; e < a + 16 && e < end; e += Elem<TYPE>::kSize)
         Elem<TYPE>::store(e, Elem<TYPE>::load(e) * c);
-    }
   }
 }
 
-// The tensor that chunk c lies in (the last whose first chunk is not behind it).
+// The descriptors, in LDS: kernel arguments lie in host memory, and a search that walks them there pays its round trip
+// at every step (a list of 100 tensors: 4 us of the launch's 13).  All of them come in one.
 template <int MOST>
-__device__ __forceinline__ int tensor_of(const GradChunks<MOST>& a, uint32_t c) {
-  int lo = 0, hi = a.count - 1;
+__device__ __forceinline__ const GradChunk* stage(const GradChunks<MOST>& a, GradChunk* s_t) {
+  static_assert(sizeof(GradChunk) == 24 && MOST * 3 <= kBlock, "three words a descriptor, a word a thread");
+  if ((int)threadIdx.x < 3 * a.count) ((uint64_t*)s_t)[threadIdx.x] = ((const uint64_t*)a.t)[threadIdx.x];
+  __syncthreads();
+  return s_t;
+}
+
+// The tensor that chunk c lies in (the last whose first chunk is not behind it).
+__device__ __forceinline__ int tensor_of(const GradChunk* t, int count, uint32_t c) {
+  int lo = 0, hi = count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (a.t[mid].first <= c) lo = mid; else hi = mid - 1;
+    if (t[mid].first <= c) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
@@ -189,13 +197,15 @@ __device__ __forceinline__ void join_block(double acc, double* out) {
 
 template <int NORM, int MOST>
 __global__ void __launch_bounds__(kBlock) norm_kernel(GradChunks<MOST> a, double* __restrict__ partials) {
+  __shared__ GradChunk s_t[MOST];
+  const GradChunk* t = stage(a, s_t);
   double acc = 0.0;
-  int k = tensor_of(a, blockIdx.x);
+  int k = tensor_of(t, a.count, blockIdx.x);
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    while (k + 1 < a.count && a.t[k + 1].first <= c) k++;
-    const uintptr_t begin = a.t[k].begin, end = a.t[k].end;
-    const uintptr_t base = (begin & ~(uintptr_t)15) + (uintptr_t)(c - a.t[k].first) * kChunk;
-    switch (a.t[k].type) {
+    while (k + 1 < a.count && t[k + 1].first <= c) k++;
+    const uintptr_t begin = t[k].begin, end = t[k].end;
+    const uintptr_t base = (begin & ~(uintptr_t)15) + (uintptr_t)(c - t[k].first) * kChunk;
+    switch (t[k].type) {
       case GSR_F32: acc = add_chunk<NORM, GSR_F32>(acc, base, begin, end); break;
       case GSR_F16: acc = add_chunk<NORM, GSR_F16>(acc, base, begin, end); break;
       default: acc = add_chunk<NORM, GSR_BF16>(acc, base, begin, end); break;
@@ -218,7 +228,8 @@ __global__ void __launch_bounds__(64) norm_final_kernel(const double* __restrict
   if (threadIdx.x == 0) *norm = (float)n;
 }
 
-// Walks the chunks backwards: what the norm pass read last is still in the last-level cache.
+// Walks the chunks backwards, eight by eight: what the norm pass read last is still in the last-level cache, and
+// chunk c falls to a workgroup of number c mod 8 in both passes, the same XCD, whose L2 may hold it.
 template <int NORM, int MOST>
 __global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks<MOST> a, const double* __restrict__ partials, int used,
                                                       double max_norm, float* __restrict__ norm) {
@@ -226,13 +237,17 @@ __global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks<MOST> a, const 
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
   const float coefficient = gsr::clip_coefficient(n, max_norm);
   if (coefficient == 1.0f) return;                           // x * 1 is x: nothing to write
-  int k = tensor_of(a, a.chunks - 1 - blockIdx.x);
-  for (uint32_t i = blockIdx.x; i < a.chunks; i += gridDim.x) {
-    const uint32_t c = a.chunks - 1 - i;
-    while (a.t[k].first > c) k--;
-    const uintptr_t begin = a.t[k].begin, end = a.t[k].end;
-    const uintptr_t base = (begin & ~(uintptr_t)15) + (uintptr_t)(c - a.t[k].first) * kChunk;
-    switch (a.t[k].type) {
+  __shared__ GradChunk s_t[MOST];
+  const GradChunk* t = stage(a, s_t);
+  const uint32_t eights = (a.chunks + 7) / 8;
+  int k = a.count - 1;
+  for (uint32_t i = blockIdx.x; i < eights * 8; i += gridDim.x) {
+    const uint32_t c = (eights - 1 - i / 8) * 8 + i % 8;
+    if (c >= a.chunks) continue;
+    if (t[k].first > c) k = tensor_of(t, k, c);              // one of those before
+    const uintptr_t begin = t[k].begin, end = t[k].end;
+    const uintptr_t base = (begin & ~(uintptr_t)15) + (uintptr_t)(c - t[k].first) * kChunk;
+    switch (t[k].type) {
       case GSR_F32: scale_chunk<GSR_F32>(coefficient, base, begin, end); break;
       case GSR_F16: scale_chunk<GSR_F16>(coefficient, base, begin, end); break;
       default: scale_chunk<GSR_BF16>(coefficient, base, begin, end); break;
@@ -288,7 +303,7 @@ int launch_clip(int count, const GsrGrad* h_grads, int norm_type, const double* 
   for (int at = 0; at < count;) {
     fill(a, count, h_grads, &at);
     if (!a.chunks) continue;
-    const dim3 grid(std::min<uint32_t>(a.chunks, kClipBlocks)), block(kBlock);
+    const dim3 grid(std::min<uint32_t>((a.chunks + 7) / 8 * 8, kClipBlocks)), block(kBlock);
     if (norm_type == GSR_NORM_2)
       hipLaunchKernelGGL((clip_kernel<GSR_NORM_2, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm);
     else if (norm_type == GSR_NORM_1)
