@@ -18,6 +18,7 @@
 
 namespace {
 
+using gsr::global_at;
 using gsr::kGradsPerLaunch;
 using gsr::kNormBlocks;
 
@@ -64,20 +65,20 @@ struct Elem;
 template <>
 struct Elem<GSR_F32> {
   static constexpr int kSize = 4;
-  __device__ static __forceinline__ float load(uintptr_t a) { return *(const float*)a; }
-  __device__ static __forceinline__ void store(uintptr_t a, float v) { *(float*)a = v; }
+  __device__ static __forceinline__ float load(uintptr_t a) { return *global_at<const float>(a); }
+  __device__ static __forceinline__ void store(uintptr_t a, float v) { *global_at<float>(a) = v; }
 };
 template <>
 struct Elem<GSR_F16> {
   static constexpr int kSize = 2;
-  __device__ static __forceinline__ float load(uintptr_t a) { return f16_to_f32(*(const uint16_t*)a); }
-  __device__ static __forceinline__ void store(uintptr_t a, float v) { *(uint16_t*)a = (uint16_t)f32_to_f16(v); }
+  __device__ static __forceinline__ float load(uintptr_t a) { return f16_to_f32(*global_at<const uint16_t>(a)); }
+  __device__ static __forceinline__ void store(uintptr_t a, float v) { *global_at<uint16_t>(a) = (uint16_t)f32_to_f16(v); }
 };
 template <>
 struct Elem<GSR_BF16> {
   static constexpr int kSize = 2;
-  __device__ static __forceinline__ float load(uintptr_t a) { return bf16_to_f32(*(const uint16_t*)a); }
-  __device__ static __forceinline__ void store(uintptr_t a, float v) { *(uint16_t*)a = (uint16_t)f32_to_bf16(v); }
+  __device__ static __forceinline__ float load(uintptr_t a) { return bf16_to_f32(*global_at<const uint16_t>(a)); }
+  __device__ static __forceinline__ void store(uintptr_t a, float v) { *global_at<uint16_t>(a) = (uint16_t)f32_to_bf16(v); }
 };
 
 template <int NORM>
@@ -112,7 +113,7 @@ __device__ __forceinline__ double add_chunk(double acc, uintptr_t base, uintptr_
 #pragma unroll
   for (int r = 0; r < kRounds; r++) {
     const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
-    v[r] = a >= begin && a + 16 <= end ? *(const u4*)a : (u4){0, 0, 0, 0};     // zeros add nothing
+    v[r] = a >= begin && a + 16 <= end ? *global_at<const u4>(a) : (u4){0, 0, 0, 0};     // zeros add nothing
   }
 #pragma unroll
   for (int r = 0; r < kRounds; r++) acc = add_vector<NORM, TYPE>(acc, v[r]);
@@ -146,12 +147,12 @@ __device__ __forceinline__ void scale_chunk(float c, uintptr_t base, uintptr_t b
 #pragma unroll
   for (int r = 0; r < kRounds; r++) {
     const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
-    v[r] = a >= begin && a + 16 <= end ? *(const u4*)a : (u4){0, 0, 0, 0};
+    v[r] = a >= begin && a + 16 <= end ? *global_at<const u4>(a) : (u4){0, 0, 0, 0};
   }
 #pragma unroll
   for (int r = 0; r < kRounds; r++) {
     const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
-    if (a >= begin && a + 16 <= end) *(u4*)a = scale_vector<TYPE>(v[r], c);
+    if (a >= begin && a + 16 <= end) *global_at<u4>(a) = scale_vector<TYPE>(v[r], c);
   }
   if (base >= begin && base + kChunk <= end) return;
   for (int r = 0; r < kRounds; r++) {

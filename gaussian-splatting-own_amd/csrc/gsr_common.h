@@ -62,6 +62,13 @@ inline Pack make_pack(int P, int tiles_x, int tiles_y) {
   return k;
 }
 
+// An address kept as a number, as a pointer to global memory: from a bare cast the compiler makes flat accesses, which
+// count as LDS accesses too and wait for them.
+template <typename T>
+__device__ __forceinline__ T __attribute__((address_space(1)))* global_at(uintptr_t at) {
+  return (T __attribute__((address_space(1)))*)at;
+}
+
 // Inclusive prefix sum over the 64 lanes of a wave with DPP alone: row_shr 1, 2, 4, 8 inside the rows of 16 lanes
 // (lanes whose source lies outside their row add nothing), then lane 15 of rows 0 and 2 into the rows behind them,
 // then lane 31 into rows 2 and 3.  Six dependent register operations; the same scan with __shfl_up is six round

@@ -41,7 +41,8 @@ struct Moves {
     char* out;
     uint64_t row_bytes;
     Divisor units;                                 // units of a row
-    uint32_t unit;                                 // bytes of a unit: what rows, their length and the pointers are multiples of
+    uint16_t unit;                                 // bytes of a unit: what rows, their length and the pointers are multiples of
+    uint16_t wide;                                 // lies_in_two_rows
     uint32_t first_block;
   } t[kRowsPerLaunch];
   int count;
@@ -50,13 +51,20 @@ struct Moves {
 };
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-// 16 bytes at a multiple of 4: the hardware's wide accesses ask for no more
-typedef uint32_t u4_4 __attribute__((ext_vector_type(4), aligned(4)));
-
+// A unit, and 16 bytes at any multiple of one: global memory takes wide accesses at every byte.
 template <int U> struct Unit;
-template <> struct Unit<4> { typedef uint32_t type; };
-template <> struct Unit<2> { typedef uint16_t type; };
-template <> struct Unit<1> { typedef uint8_t type; };
+template <> struct Unit<4> { typedef uint32_t type; typedef uint32_t wide __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Unit<2> { typedef uint16_t type; typedef uint32_t wide __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Unit<1> { typedef uint8_t type; typedef uint32_t wide __attribute__((ext_vector_type(4), aligned(1))); };
+
+template <int U>
+__device__ __forceinline__ u4 load_wide(const char* at) {
+  return __builtin_nontemporal_load((const typename Unit<U>::wide*)at);
+}
+template <int U>
+__device__ __forceinline__ void store_wide(char* at, u4 v) {
+  __builtin_nontemporal_store((typename Unit<U>::wide)v, (typename Unit<U>::wide*)at);
+}
 
 // Where a row of the concatenation lies, and its number within its own buffer of `of` rows; `at` is null for a row of
 // zeros, which an index that is negative or behind the last row stands for.
@@ -79,14 +87,29 @@ template <int U, typename I>
 __device__ __forceinline__ void move_units(const Moves& a, const Moves::One& t, uint64_t unit, uint64_t total, uint32_t row,
                                            uint32_t col) {
   typedef typename Unit<U>::type T;
-  for (int k = 0; k < 16 / U && unit + k < total; k++) {
-    const Place p = place_of(a, t, ((const I*)a.index)[row]);
-    ((T*)t.out)[unit + k] = p.at ? *(const T*)(p.at + (uint64_t)col * U) : (T)0;
+  constexpr int K = 16 / U;
+  T v[K];
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    v[k] = 0;
+    if (row < a.n_out) {
+      const Place p = place_of(a, t, ((const I*)a.index)[row]);
+      if (p.at) v[k] = *(const T*)(p.at + (uint64_t)col * U);
+    }
     if (++col == t.units.d) { col = 0; row++; }
+  }
+  if (unit + K <= total) {
+    u4 all;
+    __builtin_memcpy(&all, v, 16);
+    store_wide<U>(t.out + unit * U, all);
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; k++)
+      if (unit + k < total) ((T*)t.out)[unit + k] = v[k];
   }
 }
 
-// One workgroup's vectors of tensor `t`.
+// One workgroup's vectors of tensor `t`: rows so short that a vector may lie in three or more of them.
 template <int U, typename I>
 __device__ __forceinline__ void move_block(const Moves& a, const Moves::One& t, uint32_t block) {
   constexpr int K = 16 / U;                                              // units of a vector
@@ -101,23 +124,30 @@ __device__ __forceinline__ void move_block(const Moves& a, const Moves::One& t, 
   }
 }
 
-// The same in units of 4 bytes, the ordinary case.  A vector lies in one row or in the ends of two (rows of a single
-// unit apart): one wide load from where it begins, past the end of that row if it is split, and where the second row
-// does not happen to follow the first in memory another, from as far before it.  The loads of all rounds go out
-// before the first store.
-template <typename I>
+// Whether a vector, which begins at a multiple of K units of the output, never reaches into a third row: column and
+// length together stay below two rows.  All rows of 15 bytes and more, and those that divide a vector in half.
+inline bool lies_in_two_rows(uint32_t units, uint32_t unit) {
+  const uint32_t k = 16 / unit;
+  return units + k - 2 < 2 * units || 2 * units == k;
+}
+
+// The same for rows that lies_in_two_rows holds for, the ordinary case.  One wide load from where the vector begins,
+// past the end of its row if it is split, and where the second row does not happen to follow the first in memory
+// another, from as far before that.  The loads of all rounds go out before the first store.
+template <int U, typename I>
 __device__ __forceinline__ void move_block_wide(const Moves& a, const Moves::One& t, uint32_t block) {
+  constexpr uint32_t K = 16 / U;
   const I* index = (const I*)a.index;
   const uint32_t w = t.units.d;
   const uint64_t total = (uint64_t)a.n_out * w;
-  const uint64_t first = (uint64_t)block * kPerBlock * 4;
+  const uint64_t first = (uint64_t)block * kPerBlock * K;
   const uint32_t row0 = (uint32_t)(first / w), col0 = (uint32_t)(first % w);
   uint32_t row[kRounds], col[kRounds];
   I i0[kRounds], i1[kRounds];
   u4 v[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; r++) {
-    const uint32_t at = (uint32_t)(r * kBlock + threadIdx.x) * 4;
+    const uint32_t at = (uint32_t)(r * kBlock + threadIdx.x) * K;
     const uint32_t over = t.units.quotient(col0 + at);
     row[r] = row0 + over;
     col[r] = col0 + at - over * w;
@@ -127,25 +157,35 @@ __device__ __forceinline__ void move_block_wide(const Moves& a, const Moves::One
   bool whole[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; r++) {
-    const uint64_t unit = first + (uint32_t)(r * kBlock + threadIdx.x) * 4;
-    const uint32_t here = w - col[r];                                    // units of the vector in its first row, if below 4
+    const uint64_t unit = first + (uint32_t)(r * kBlock + threadIdx.x) * K;
+    const uint32_t here = w - col[r];                                    // units of the vector in its first row, if below K
     const Place p = place_of(a, t, i0[r]), q = place_of(a, t, i1[r]);
-    const bool split = here < 4, follows = p.at && q.at == p.at + t.row_bytes;
+    const bool split = here < K, follows = p.at && q.at == p.at + t.row_bytes;
     // a wide load must not leave its buffer: behind the last row, or before the first
-    whole[r] = unit + 4 <= total && !(split && ((p.at && p.row + 1 == p.of) || (q.at && !follows && q.row == 0)));
+    whole[r] = unit + K <= total && !(split && ((p.at && p.row + 1 == p.of) || (q.at && !follows && q.row == 0)));
     u4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-    if (whole[r] && p.at) x = __builtin_nontemporal_load((const u4_4*)(p.at + (uint64_t)col[r] * 4));
-    if (whole[r] && split && !follows && q.at) y = __builtin_nontemporal_load((const u4_4*)(q.at - (uint64_t)here * 4));
-    const uint32_t from_first = follows ? 4 : here;
+    if (whole[r] && p.at) x = load_wide<U>(p.at + (uint64_t)col[r] * U);
+    if (whole[r] && split && !follows && q.at) y = load_wide<U>(q.at - (uint64_t)here * U);
+    const int from_first = follows || !split ? 16 : (int)here * U;       // bytes
 #pragma unroll
-    for (int k = 0; k < 4; k++) v[r][k] = (uint32_t)k < from_first ? x[k] : y[k];
+    for (int k = 0; k < 4; k++) {
+      const int n = from_first - 4 * k;                                  // of them in word k
+      const uint32_t mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+      v[r][k] = (x[k] & mask) | (y[k] & ~mask);
+    }
   }
 #pragma unroll
   for (int r = 0; r < kRounds; r++) {
-    const uint64_t unit = first + (uint32_t)(r * kBlock + threadIdx.x) * 4;
-    if (whole[r]) __builtin_nontemporal_store((u4_4)v[r], (u4_4*)((uint32_t*)t.out + unit));
-    else if (unit < total) move_units<4, I>(a, t, unit, total, row[r], col[r]);
+    const uint64_t unit = first + (uint32_t)(r * kBlock + threadIdx.x) * K;
+    if (whole[r]) store_wide<U>(t.out + unit * U, v[r]);
+    else if (unit < total) move_units<U, I>(a, t, unit, total, row[r], col[r]);
   }
+}
+
+template <int U, typename I>
+__device__ __forceinline__ void move(const Moves& a, const Moves::One& t, uint32_t block) {
+  if (t.wide) move_block_wide<U, I>(a, t, block);
+  else move_block<U, I>(a, t, block);
 }
 
 template <typename I>
@@ -154,10 +194,9 @@ __global__ void __launch_bounds__(kBlock) move_kernel(Moves a) {
   while (k + 1 < a.count && blockIdx.x >= a.t[k + 1].first_block) k++;
   const Moves::One t = a.t[k];
   const uint32_t block = blockIdx.x - t.first_block;
-  if (t.unit == 4 && t.units.d > 1) move_block_wide<I>(a, t, block);
-  else if (t.unit == 4) move_block<4, I>(a, t, block);
-  else if (t.unit == 2) move_block<2, I>(a, t, block);
-  else move_block<1, I>(a, t, block);
+  if (t.unit == 4) move<4, I>(a, t, block);
+  else if (t.unit == 2) move<2, I>(a, t, block);
+  else move<1, I>(a, t, block);
 }
 
 // ---- positions of the kept rows ----
@@ -181,12 +220,12 @@ __device__ __forceinline__ uint32_t flags_of(const Flags& f, uint32_t tile) {
   if (at >= f.end) return 0;
   uint32_t bits = 0;
   if (at >= f.skip && at + 16 <= f.end) {
-    const u4 v = *(const u4*)(f.base + at);
+    const u4 v = *gsr::global_at<const u4>(f.base + at);
 #pragma unroll
     for (int b = 0; b < 16; b++) bits |= ((v[b >> 2] >> (8 * (b & 3))) & 0xffu ? 1u : 0u) << b;
   } else {
     for (int b = 0; b < 16; b++)
-      if (at + b >= f.skip && at + b < f.end && *(const uint8_t*)(f.base + at + b)) bits |= 1u << b;
+      if (at + b >= f.skip && at + b < f.end && *gsr::global_at<const uint8_t>(f.base + at + b)) bits |= 1u << b;
   }
   return bits;
 }
@@ -320,6 +359,7 @@ extern "C" int gsr_select_rows(int count, const GsrRows* h_tensors, uint64_t n_r
       u.unit = 4;
       while ((align | t.row_bytes) % u.unit) u.unit >>= 1;
       u.units = divisor((uint32_t)(t.row_bytes / u.unit));
+      u.wide = lies_in_two_rows(u.units.d, u.unit);
       u.first_block = (uint32_t)blocks;
       blocks += all;
     }

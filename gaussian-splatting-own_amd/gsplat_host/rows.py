@@ -46,6 +46,9 @@ def _checked(tensors: Sequence[torch.Tensor]) -> Tuple[List[torch.Tensor], torch
 
 
 def _contiguous(tensors: Sequence[Optional[torch.Tensor]]) -> List[Optional[torch.Tensor]]:
+    """Rows whose bytes are the values: in order, without gaps, and no conjugation or sign left for later."""
+    if any(t is not None and (t.is_conj() or t.is_neg()) for t in tensors):
+        tensors = [None if t is None else t.detach().resolve_conj().resolve_neg() for t in tensors]
     return [t if t is None or t.is_contiguous() else t.detach().contiguous() for t in tensors]
 
 
