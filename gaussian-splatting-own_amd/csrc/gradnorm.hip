@@ -25,6 +25,9 @@ using gsr::kNormBlocks;
 constexpr int kBlock = 512;
 constexpr int kRounds = 4;                                   // 16-byte accesses of a thread in flight
 constexpr uint32_t kChunk = kBlock * kRounds * 16;           // bytes
+// Gradients beyond the size of the last-level cache are scaled past it: with the norm pass, 472 MB of fp32 take 236 us
+// so and 262 through it, 1.4 GB 768 and 821; 165 MB the other way round 80 and 73, 236 MB 111 and 103.
+constexpr uint64_t kStreamBytes = 256ull << 20;
 constexpr uint32_t kClipBlocks = 1024;                       // workgroups of a clipping launch at most
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -140,19 +143,23 @@ __device__ __forceinline__ u4 scale_vector(u4 v, float c) {
   return o;
 }
 
-template <int TYPE>
+// STREAM: past the caches (kStreamBytes).
+template <int TYPE, bool STREAM>
 __device__ __forceinline__ void scale_chunk(float c, uintptr_t base, uintptr_t begin, uintptr_t end) {
   const uintptr_t mine = base + threadIdx.x * 16u;
   u4 v[kRounds];
 #pragma unroll
   for (int r = 0; r < kRounds; r++) {
     const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
-    v[r] = a >= begin && a + 16 <= end ? *global_at<const u4>(a) : (u4){0, 0, 0, 0};
+    v[r] = (u4){0, 0, 0, 0};
+    if (a >= begin && a + 16 <= end) v[r] = STREAM ? __builtin_nontemporal_load(global_at<const u4>(a)) : *global_at<const u4>(a);
   }
 #pragma unroll
   for (int r = 0; r < kRounds; r++) {
     const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
-    if (a >= begin && a + 16 <= end) *global_at<u4>(a) = scale_vector<TYPE>(v[r], c);
+    if (a < begin || a + 16 > end) continue;
+    if (STREAM) __builtin_nontemporal_store(scale_vector<TYPE>(v[r], c), global_at<u4>(a));
+    else *global_at<u4>(a) = scale_vector<TYPE>(v[r], c);
   }
   if (base >= begin && base + kChunk <= end) return;
   for (int r = 0; r < kRounds; r++) {
@@ -233,7 +240,7 @@ __global__ void __launch_bounds__(64) norm_final_kernel(const double* __restrict
 // chunk c falls to a workgroup of number c mod 8 in both passes, the same XCD, whose L2 may hold it.
 template <int NORM, int MOST>
 __global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks<MOST> a, const double* __restrict__ partials, int used,
-                                                      double max_norm, float* __restrict__ norm) {
+                                                      double max_norm, float* __restrict__ norm, int stream) {
   const double n = gsr::norm_of_partials<NORM>(partials, used);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
   const float coefficient = gsr::clip_coefficient(n, max_norm);
@@ -248,10 +255,13 @@ __global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks<MOST> a, const 
     if (t[k].first > c) k = tensor_of(t, k, c);              // one of those before
     const uintptr_t begin = t[k].begin, end = t[k].end;
     const uintptr_t base = (begin & ~(uintptr_t)15) + (uintptr_t)(c - t[k].first) * kChunk;
-    switch (t[k].type) {
-      case GSR_F32: scale_chunk<GSR_F32>(coefficient, base, begin, end); break;
-      case GSR_F16: scale_chunk<GSR_F16>(coefficient, base, begin, end); break;
-      default: scale_chunk<GSR_BF16>(coefficient, base, begin, end); break;
+    switch (t[k].type + (stream ? 4u : 0u)) {
+      case GSR_F32: scale_chunk<GSR_F32, false>(coefficient, base, begin, end); break;
+      case GSR_F16: scale_chunk<GSR_F16, false>(coefficient, base, begin, end); break;
+      case GSR_BF16: scale_chunk<GSR_BF16, false>(coefficient, base, begin, end); break;
+      case GSR_F32 + 4: scale_chunk<GSR_F32, true>(coefficient, base, begin, end); break;
+      case GSR_F16 + 4: scale_chunk<GSR_F16, true>(coefficient, base, begin, end); break;
+      default: scale_chunk<GSR_BF16, true>(coefficient, base, begin, end); break;
     }
   }
 }
@@ -300,17 +310,20 @@ int launch_norm(int count, const GsrGrad* h_grads, int norm_type, double* partia
 template <int MOST>
 int launch_clip(int count, const GsrGrad* h_grads, int norm_type, const double* partials, int used, double max_norm,
                 float* norm, hipStream_t stream) {
+  uint64_t chunks = 0;
+  for (int k = 0; k < count; k++) chunks += chunks_of(h_grads[k]);
+  const bool stream_past = chunks > kStreamBytes / kChunk;
   GradChunks<MOST> a;
   for (int at = 0; at < count;) {
     fill(a, count, h_grads, &at);
     if (!a.chunks) continue;
     const dim3 grid(std::min<uint32_t>((a.chunks + 7) / 8 * 8, kClipBlocks)), block(kBlock);
     if (norm_type == GSR_NORM_2)
-      hipLaunchKernelGGL((clip_kernel<GSR_NORM_2, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm);
+      hipLaunchKernelGGL((clip_kernel<GSR_NORM_2, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm, (int)stream_past);
     else if (norm_type == GSR_NORM_1)
-      hipLaunchKernelGGL((clip_kernel<GSR_NORM_1, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm);
+      hipLaunchKernelGGL((clip_kernel<GSR_NORM_1, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm, (int)stream_past);
     else
-      hipLaunchKernelGGL((clip_kernel<GSR_NORM_MAX, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm);
+      hipLaunchKernelGGL((clip_kernel<GSR_NORM_MAX, MOST>), grid, block, 0, stream, a, partials, used, max_norm, norm, (int)stream_past);
     const int rc = gsr::check_launch("clip_grads");
     if (rc != GSR_OK) return rc;
     norm = nullptr;                                          // the first launch has written it

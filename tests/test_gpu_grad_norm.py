@@ -432,3 +432,20 @@ def test_lists_whose_partial_results_are_joined_first():
     bound = 0.2 * norm64([before], 2.0)
     check_norm(clip_grads_(tensors, bound), [before], 2.0)
     check_clipped(pool, before, factor64(norm64([before], 2.0), bound))
+
+
+def test_gradients_beyond_the_last_level_cache():
+    """Over 256 MiB, which are scaled past the caches: all three types, at odd alignments and of odd sizes."""
+    from gsplat_host.optim import clip_grads_
+    sizes = [(40_000_003, torch.float32), (1, torch.float16), (30_000_001, torch.bfloat16), (25_165_827, torch.float16), (77, torch.float32)]
+    pools = [values(n + 3, t, k) for k, (n, t) in enumerate(sizes)]
+    tensors = [p[1 + k % 2:1 + k % 2 + n] for k, (p, (n, _)) in enumerate(zip(pools, sizes))]
+    assert sum(t.numel() * t.element_size() for t in tensors) > 256 << 20
+    before = [p.clone() for p in pools]
+    inside = [b[1 + k % 2:1 + k % 2 + n] for k, (b, (n, _)) in enumerate(zip(before, sizes))]
+    norm = norm64(inside, 2.0)
+    check_norm(clip_grads_(tensors, 0.4 * norm), inside, 2.0)
+    for k, (t, b, p, whole) in enumerate(zip(tensors, inside, pools, before)):
+        check_clipped(t, b, factor64(norm, 0.4 * norm))
+        at = 1 + k % 2
+        assert torch.equal(p[:at], whole[:at]) and torch.equal(p[at + t.numel():], whole[at + t.numel():])

@@ -138,6 +138,85 @@ def test_strides_and_alignments():
     assert same(compact_rows(old[:1], strided)[0][0], old[0][strided])
 
 
+@pytest.mark.parametrize("offset", (0, 1, 2, 3))
+def test_row_lengths(offset):
+    """Rows of 1 to 40 bytes at every alignment, with first and last rows next to one another and apart."""
+    from gsplat_host.rows import compact_rows, select_rows
+    n = 203
+    for length in range(1, 41):
+        t = data(n * length + 4, (), torch.uint8, length)[offset:offset + n * length].view(n, length)
+        e = data(17 * length + 4, (), torch.uint8, 99 + length)[offset:offset + 17 * length].view(17, length)
+        g = torch.Generator(device="cuda").manual_seed(length)
+        index = torch.randint(0, n, (1009,), generator=g, device="cuda")
+        index[::7], index[1::7], index[2::7] = n - 1, 0, n - 2
+        index[500:700] = torch.arange(200, device="cuda")
+        index[3::50] = -1
+        assert same(select_rows([t], index)[0], pick(t, index)), length
+        keep = torch.rand((n + 17,), generator=g, device="cuda") < 0.8
+        keep[n - 2:n + 2] = True                                 # across the seam of the two buffers
+        for more in (e, None):
+            out, = compact_rows([t], keep, [more])[0]
+            assert same(out, torch.cat((t, torch.zeros_like(e) if more is None else more))[keep]), (length, more is None)
+
+
+def test_views_that_only_look_conjugated_or_negated():
+    from gsplat_host.rows import select_rows
+    z = torch.randn(50, 3, dtype=torch.complex64, device="cuda")
+    index = torch.tensor([4, 49, 0, 4], device="cuda")
+    for t in (z, z.conj(), z.conj().imag, z.imag, z.resolve_conj().real):
+        out, = select_rows([t], index)
+        assert torch.equal(out, t[index]) and not out.is_conj() and not out.is_neg()
+
+
+def test_compaction_refuses_to_be_captured():
+    from gsplat_host.rows import compact_rows
+    t, keep = torch.zeros((40, 3), device="cuda"), torch.ones(40, dtype=torch.bool, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            compact_rows([t], keep)
+        t.add_(1.0)                                              # a graph of something
+        graph.capture_end()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(compact_rows([t], keep)[0][0], t)
+
+
+def test_two_threads_on_streams_of_their_own():
+    """Both compact and clip at once: nothing is shared between their calls."""
+    import threading
+    from gsplat_host.optim import clip_grads_
+    from gsplat_host.rows import compact_rows
+    problems = []
+
+    def work(seed):
+        try:
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in range(30):
+                    n = 1000 + 977 * k + seed
+                    t, keep = torch.rand((n, 5), generator=g, device="cuda"), torch.rand((n,), generator=g, device="cuda") < 0.5
+                    (out,), index = compact_rows([t], keep)
+                    want = t[keep]
+                    norm = clip_grads_([t], 1.0)
+                    kept = t[keep]
+                    if not (same(out, want) and torch.equal(index.long(), keep.nonzero().view(-1))
+                            and torch.allclose(kept * norm, want, rtol=1e-5, atol=0)):   # factor, product and this one: 4 x 2^-24
+                        problems.append((seed, k))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                   # reported by the main thread
+            problems.append((seed, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not problems, problems
+
+
 def test_past_32_bits():
     """A tensor of 4.4 GB: rows that lie, and land, behind 2^32 bytes."""
     from gsplat_host.rows import compact_rows, select_rows
