@@ -20,7 +20,10 @@
 // gsr_adam_step_clipped is the same update with the gradients' norm and the bound on it in front: a norm pass
 // (gradnorm.hip) and ONE update launch whose waves join its partial results while their own loads are under way, so
 // that the clipped gradients are never written and no kernel of a single workgroup stands between the two.  It reads
-// each gradient twice: 4 B (2 B for a 16-bit one) on top of the 28 B an element.
+// each gradient twice: 4 B (2 B for a 16-bit one) on top of the 28 B an element.  6M Gaussians: 1963 us, the norm pass's
+// 227 and the plain step's 1740 (11.3 GB, 5.8 TB/s); 1M with bf16 gradients 281.  Walking the tensors backwards, as the
+// clip does, or loading the gradients through the caches changes nothing here (1957 to 2007 us; 1M in fp32 307 to 313):
+// the parameters and moments pass through the last-level cache in between.
 #include "gradnorm.h"
 
 namespace {
@@ -263,7 +266,7 @@ extern "C" int gsr_adam_step_clipped(int count, const GsrAdamTensor* h_tensors, 
     blocks += (t.n + kPerBlock - 1) / kPerBlock;
     a.count++;
   }
-  GSR_REQUIRE(blocks < ((uint64_t)1 << 31), "adam_step_clipped: too many elements");
+  GSR_REQUIRE(blocks < ((uint64_t)1 << 24), "adam_step_clipped: too many elements");     // fewer than 2^32 threads
   a.first_block[a.count] = (uint32_t)blocks;
   if (blocks == 0) return gsr_grad_norm(0, nullptr, norm_type, norm, scratch, scratch_bytes, stream);   // writes 0
   ClipArgs clip = {(const double*)scratch, 0, skip_nonfinite, max_norm, norm};

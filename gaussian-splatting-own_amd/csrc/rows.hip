@@ -9,6 +9,8 @@
 // Both are bound by HBM.  The copy works on the OUTPUT: a thread fills 16 contiguous bytes of it, wherever its rows
 // begin, and finds row and column by one multiplication (division by the row's length); with short rows (3, 12, 16, 180
 // bytes) that keeps every store full and the loads of a wave in few cache lines, which one wave a row would not.
+// 18 tensors of 6.3M rows, 90 % kept, 7.9 GB: 1423 us, 5.6 TB/s.  One row in ten of a million, six tensors: 21 us for
+// 48 MB of rows, which are 96 MB of the 128-byte lines that they lie in.
 #include <algorithm>
 
 #include "gsr_common.h"
@@ -241,8 +243,8 @@ __global__ void __launch_bounds__(kBlock) keep_count_kernel(Flags f, uint32_t* _
   if (threadIdx.x == 0) counts[blockIdx.x] = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
 }
 
-// A tile's positions meet in LDS and leave it as full lines; written by the threads that find them they are single
-// words all over a tile's stretch (6.3M flags, 90 % kept: 31 us).
+// A tile's positions meet in LDS and leave it as full lines (6.3M flags, 90 % kept: 14 us); written by the threads that
+// find them they are single words all over a tile's stretch (31 us).
 __global__ void __launch_bounds__(kBlock) keep_write_kernel(Flags f, const uint32_t* __restrict__ counts,
                                                             int32_t* __restrict__ index, uint64_t* landing, uint32_t ticket) {
   __shared__ uint32_t s_wave[kBlock / 64];
@@ -280,6 +282,8 @@ __global__ void __launch_bounds__(kBlock) keep_write_kernel(Flags f, const uint3
 }
 
 constexpr uint64_t kMostRows = 0x7fff0000ull;      // row numbers are 32-bit signed, with room to round up
+
+constexpr uint64_t kMostMoveBlocks = 0xffffffull;  // a launch has fewer than 2^32 threads: 137 GB of rows
 
 Divisor divisor(uint32_t d) {
   Divisor v = {d, 0, 0};
@@ -325,7 +329,7 @@ extern "C" int gsr_keep_rows(uint64_t n, const uint8_t* keep, int32_t* index, ui
 extern "C" int gsr_select_rows(int count, const GsrRows* h_tensors, uint64_t n_rows, uint64_t n_appended, uint64_t n_out,
                                const void* index, int index_bytes, void* stream) {
   GSR_REQUIRE(count >= 0 && (count == 0 || h_tensors), "select_rows: %d tensors, list %p", count, (const void*)h_tensors);
-  GSR_REQUIRE(n_rows + n_appended <= kMostRows && n_rows <= kMostRows && n_out <= kMostRows,
+  GSR_REQUIRE(n_rows <= kMostRows && n_appended <= kMostRows && n_rows + n_appended <= kMostRows && n_out <= kMostRows,
               "select_rows: %llu of %llu + %llu rows", (unsigned long long)n_out, (unsigned long long)n_rows,
               (unsigned long long)n_appended);
   GSR_REQUIRE(index_bytes == 4 || index_bytes == 8, "select_rows: an index of %d bytes", index_bytes);
@@ -335,6 +339,7 @@ extern "C" int gsr_select_rows(int count, const GsrRows* h_tensors, uint64_t n_r
     if (t.row_bytes == 0 || n_out == 0) continue;
     GSR_REQUIRE(t.row_bytes < (1ull << 31), "select_rows: tensor %d has rows of %zu bytes", k, t.row_bytes);
     GSR_REQUIRE(t.out && (t.rows || n_rows == 0), "select_rows: null pointer in tensor %d", k);
+    GSR_REQUIRE(n_out * t.row_bytes <= kMostMoveBlocks * 16ull * kPerBlock, "select_rows: tensor %d is too large", k);
   }
   Moves a;
   a.n_rows = (uint32_t)n_rows;
@@ -348,8 +353,7 @@ extern "C" int gsr_select_rows(int count, const GsrRows* h_tensors, uint64_t n_r
       const GsrRows& t = h_tensors[at];
       if (t.row_bytes == 0) continue;
       const uint64_t all = (n_out * t.row_bytes + 16ull * kPerBlock - 1) / (16ull * kPerBlock);
-      if (blocks && blocks + all > 0x7fffffffull) break;
-      GSR_REQUIRE(all <= 0x7fffffffull, "select_rows: tensor %d is too large", at);
+      if (blocks && blocks + all > kMostMoveBlocks) break;
       Moves::One& u = a.t[a.count++];
       u.rows = (const char*)t.rows;
       u.appended = n_appended ? (const char*)t.appended : nullptr;

@@ -4,7 +4,8 @@ The reference steps ``torch.optim.Adam`` over six parameter tensors with one
 learning rate each and ``eps = 1e-15`` (``scene/gaussian_model.py:154-163``,
 ``train.py:126-128``) and decays the position learning rate log-linearly
 (``:164-175``, ``utils/general_utils.py:29-62``).  Here the update of all six
-tensors is ONE fused HIP launch (``gsr_adam_step``), and, when several ranks
+tensors is ONE fused HIP launch (``gsr_adam_step``; with the gradients' norm bounded first two,
+``gsr_adam_step_clipped``), and, when several ranks
 each render their own view of a replicated model, their gradients meet in one
 flat buffer that is summed over the ranks (reduce-scatter + all-gather over RCCL) before the step.  There is no
 CPU path for the update: the parameters must live on the GPU.
@@ -381,7 +382,7 @@ class GaussianAdam:
     def _moves_rows_on_the_gpu(self, keep: torch.Tensor) -> bool:
         """Whether ``keep`` and every tensor are what ``compact_rows`` moves: one bool per row, on one GPU."""
         state = [t for group in (self.params, self.exp_avg, self.exp_avg_sq) for t in group.values()]
-        return (keep.dtype == torch.bool and keep.dim() == 1 and keep.is_cuda
+        return (len(state) > 0 and keep.dtype == torch.bool and keep.dim() == 1 and keep.is_cuda
                 and all(t.device == keep.device and t.dim() > 0 and t.shape[0] == keep.shape[0] for t in state))
 
     @torch.no_grad()
@@ -476,7 +477,9 @@ class GaussianAdam:
         ``clip_grads_`` would (``norm_type`` as there), in the same two launches and without touching the gradients,
         which may then be float32, float16 or bfloat16; the step returns the norm, a float32 scalar on the GPU.
         ``max_norm=math.inf`` only measures.  ``skip_nonfinite`` (with ``max_norm``): a step whose norm is infinite or
-        NaN leaves parameters and moments as they are; ``step_count`` counts it."""
+        NaN (in the 64 bits it is summed in, so only where an element is) leaves parameters and moments as they are;
+        ``step_count`` counts it.  A step captured into a graph repeats the bias corrections of the count it was captured
+        with."""
         for name, p in self.params.items():
             if not p.is_cuda:
                 raise ValueError(f"{name}: the fused update runs on the GPU only, the parameter is on {p.device}")

@@ -24,7 +24,8 @@ def select(tensors=((FAKE, 0, FAKE, 12),), n_rows=10, n_appended=0, n_out=5, ind
 def test_select_checks():
     assert select(count=-1) == -1
     assert lib.gsr_select_rows(2, None, 1, 0, 1, FAKE, 4, None) == -1
-    for kw in ({"n_rows": 1 << 31}, {"n_out": 1 << 31}, {"n_rows": 1 << 30, "n_appended": 1 << 30}, {"n_rows": (1 << 64) - 1, "n_appended": 1}):
+    for kw in ({"n_rows": 1 << 31}, {"n_out": 1 << 31}, {"n_rows": 1 << 30, "n_appended": 1 << 30}, {"n_rows": (1 << 64) - 1, "n_appended": 1},
+               {"n_rows": 1, "n_appended": (1 << 64) - 1}):
         assert select(**kw) == -1 and "rows" in last(), kw
     for nbytes in (0, 1, 2, 16):
         assert select(index_bytes=nbytes) == -1 and "index of" in last()
@@ -32,6 +33,7 @@ def test_select_checks():
     assert select(tensors=((0, 0, FAKE, 12),)) == -1 and "null pointer in tensor 0" in last()
     assert select(tensors=((FAKE, 0, FAKE, 4), (FAKE, 0, 0, 12))) == -1 and "null pointer in tensor 1" in last()
     assert select(tensors=((FAKE, 0, FAKE, 1 << 31),)) == -1 and "rows of" in last()
+    assert select(tensors=((FAKE, 0, FAKE, 1 << 30),), n_out=1 << 10) == -1 and "too large" in last()
     # nothing to do is no error, whatever the pointers
     assert select(n_out=0, index=None) == 0 and select(tensors=(), n_out=5) == 0 and select(tensors=((0, 0, 0, 0),)) == 0
 
