@@ -29,9 +29,6 @@ using gsr::kNormBlocks;
 constexpr int kBlock = 512;
 constexpr int kRounds = 4;                                   // 16-byte accesses of a thread in flight
 constexpr uint32_t kChunk = kBlock * kRounds * 16;           // bytes
-// Gradients beyond the size of the last-level cache are scaled past it: with the norm pass, 472 MB of fp32 take 236 us
-// so and 262 through it, 1.4 GB 768 and 821; 165 MB the other way round 80 and 73, 236 MB 111 and 103.
-constexpr uint64_t kStreamBytes = 256ull << 20;
 constexpr uint32_t kClipBlocks = 1024;                       // workgroups of a clipping launch at most
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -147,7 +144,7 @@ __device__ __forceinline__ u4 scale_vector(u4 v, float c) {
   return o;
 }
 
-// STREAM: past the caches (kStreamBytes).
+// STREAM: past the caches.
 template <int TYPE, bool STREAM>
 __device__ __forceinline__ void scale_chunk(float c, uintptr_t base, uintptr_t begin, uintptr_t end) {
   const uintptr_t mine = base + threadIdx.x * 16u;
@@ -318,7 +315,9 @@ int launch_clip(int count, const GsrGrad* h_grads, int norm_type, const double* 
                 float* norm, hipStream_t stream) {
   uint64_t chunks = 0;
   for (int k = 0; k < count; k++) chunks += chunks_of(h_grads[k]);
-  const bool stream_past = chunks > kStreamBytes / kChunk;
+  // Gradients beyond the size of the last-level cache are scaled past it: with the norm pass, 472 MB of fp32 take 236 us
+  // so and 262 through it, 1.4 GB 768 and 821; 165 MB the other way round 80 and 73, 236 MB 111 and 103.
+  const bool stream_past = chunks > gsr::kLastLevelBytes / kChunk;
   GradChunks<MOST> a;
   for (int at = 0; at < count;) {
     fill(a, count, h_grads, &at);

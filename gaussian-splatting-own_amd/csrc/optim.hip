@@ -20,10 +20,10 @@
 // gsr_adam_step_clipped is the same update with the gradients' norm and the bound on it in front: a norm pass
 // (gradnorm.hip) and ONE update launch whose waves join its partial results while their own loads are under way, so
 // that the clipped gradients are never written and no kernel of a single workgroup stands between the two.  It reads
-// each gradient twice: 4 B (2 B for a 16-bit one) on top of the 28 B an element.  6M Gaussians: 1963 us, the norm pass's
-// 227 and the plain step's 1740 (11.3 GB, 5.8 TB/s); 1M with bf16 gradients 281.  Walking the tensors backwards, as the
-// clip does, or loading the gradients through the caches changes nothing here (1957 to 2007 us; 1M in fp32 307 to 313):
-// the parameters and moments pass through the last-level cache in between.
+// each gradient twice: 4 B (2 B for a 16-bit one) on top of the 28 B an element.  6M Gaussians: 1880 us, 227 of them
+// the norm pass (11.3 GB, 6.0 TB/s); 1M 274, with bf16 gradients 259.  Gradients up to the size of the last-level cache
+// are read through it (1M: 274 us, nontemporally 281; 6M: 1930 and 1880).  Walking the tensors backwards, as the clip
+// does, changes nothing here: the parameters and moments pass by in between.
 #include "gradnorm.h"
 
 namespace {
@@ -114,14 +114,19 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef unsigned short us4 __attribute__((ext_vector_type(4)));
 
 // Four gradients from element `i` (aligned to four of them), and one, as fp32; the conversions are exact.
-template <int TYPE>
+template <int TYPE, bool CACHED>
 __device__ __forceinline__ f4 grads_at(const void* grad, size_t i) {
-  if (TYPE == GSR_F32) return GSR_LD((const f4*)((const float*)grad + i));
+  if (TYPE == GSR_F32) {
+    const f4* at = (const f4*)((const float*)grad + i);
+    return CACHED ? *at : GSR_LD(at);
+  }
   if (TYPE == GSR_F16) {
-    const h4 h = GSR_LD((const h4*)((const _Float16*)grad + i));
+    const h4* at = (const h4*)((const _Float16*)grad + i);
+    const h4 h = CACHED ? *at : GSR_LD(at);
     return (f4){(float)h.x, (float)h.y, (float)h.z, (float)h.w};
   }
-  const us4 h = GSR_LD((const us4*)((const unsigned short*)grad + i));
+  const us4* at = (const us4*)((const unsigned short*)grad + i);
+  const us4 h = CACHED ? *at : GSR_LD(at);
   return (f4){__uint_as_float((uint32_t)h.x << 16), __uint_as_float((uint32_t)h.y << 16),
               __uint_as_float((uint32_t)h.z << 16), __uint_as_float((uint32_t)h.w << 16)};
 }
@@ -134,7 +139,8 @@ __device__ __forceinline__ float grad_at(const void* grad, size_t i) {
 
 // One workgroup's elements of tensor `t`, whose gradient is of type TYPE.  The factor on the gradients comes after the
 // loads are issued: joining the partial results hides behind them.
-template <int NORM, int TYPE>
+// CACHED: the norm pass has left the gradients in the last-level cache, they are read through it.
+template <int NORM, int TYPE, bool CACHED>
 __device__ __forceinline__ void clipped_block(const GsrAdamTensor& t, size_t first, const ClipArgs& clip, float w1, float b2,
                                               float w2, float eps, float step_size, float inv_bc2_sqrt, float grad_scale) {
   const size_t block_base = first + (size_t)threadIdx.x * kPerThread;
@@ -145,7 +151,7 @@ __device__ __forceinline__ void clipped_block(const GsrAdamTensor& t, size_t fir
     for (int r = 0; r < kRounds; r++) {
       const size_t base = block_base + (size_t)r * kBlock * kPerThread;
       p[r] = GSR_LD(reinterpret_cast<f4*>(t.param + base));
-      g[r] = grads_at<TYPE>(t.grad, base);
+      g[r] = grads_at<TYPE, CACHED>(t.grad, base);
       m[r] = GSR_LD(reinterpret_cast<f4*>(t.exp_avg + base));
       v[r] = GSR_LD(reinterpret_cast<f4*>(t.exp_avg_sq + base));
     }
@@ -185,7 +191,7 @@ struct GradTypes {
   uint8_t of[GSR_ADAM_MAX_TENSORS];
 };
 
-template <int NORM>
+template <int NORM, bool CACHED>
 __global__ void __launch_bounds__(kBlock) adam_clipped_kernel(AdamTensors a, GradTypes types, ClipArgs clip, float w1, float b2,
                                                               float w2, float eps, float bc1, float inv_bc2_sqrt,
                                                               float grad_scale) {
@@ -195,9 +201,15 @@ __global__ void __launch_bounds__(kBlock) adam_clipped_kernel(AdamTensors a, Gra
   const size_t first = (size_t)(blockIdx.x - a.first_block[k]) * kPerBlock;
   const float step_size = t.lr / bc1;
   switch (types.of[k]) {
-    case GSR_F32: clipped_block<NORM, GSR_F32>(t, first, clip, w1, b2, w2, eps, step_size, inv_bc2_sqrt, grad_scale); break;
-    case GSR_F16: clipped_block<NORM, GSR_F16>(t, first, clip, w1, b2, w2, eps, step_size, inv_bc2_sqrt, grad_scale); break;
-    default: clipped_block<NORM, GSR_BF16>(t, first, clip, w1, b2, w2, eps, step_size, inv_bc2_sqrt, grad_scale); break;
+    case GSR_F32:
+      clipped_block<NORM, GSR_F32, CACHED>(t, first, clip, w1, b2, w2, eps, step_size, inv_bc2_sqrt, grad_scale);
+      break;
+    case GSR_F16:
+      clipped_block<NORM, GSR_F16, CACHED>(t, first, clip, w1, b2, w2, eps, step_size, inv_bc2_sqrt, grad_scale);
+      break;
+    default:
+      clipped_block<NORM, GSR_BF16, CACHED>(t, first, clip, w1, b2, w2, eps, step_size, inv_bc2_sqrt, grad_scale);
+      break;
   }
 }
 
@@ -253,10 +265,11 @@ extern "C" int gsr_adam_step_clipped(int count, const GsrAdamTensor* h_tensors, 
   if (rc != GSR_OK) return rc;
   AdamTensors a{};
   GradTypes types{};
-  uint64_t blocks = 0;
+  uint64_t blocks = 0, grad_bytes = 0;
   for (int k = 0; k < count; k++) {
     const GsrAdamTensor& t = h_tensors[k];
     if (t.n == 0) continue;
+    grad_bytes += t.n * (grads[k].type == GSR_F32 ? 4 : 2);
     GsrAdamTensor u = t;
     const uintptr_t grad_align = grads[k].type == GSR_F32 ? 15 : 7;
     u.vec4 = (((uintptr_t)t.param | (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) & 15) == 0 && ((uintptr_t)t.grad & grad_align) == 0;
@@ -274,13 +287,13 @@ extern "C" int gsr_adam_step_clipped(int count, const GsrAdamTensor* h_tensors, 
   if (rc != GSR_OK) return rc;
   const double bc1 = 1.0 - pow(beta1, (double)step);
   const double bc2_sqrt = sqrt(1.0 - pow(beta2, (double)step));
-#define GSR_LAUNCH_CLIPPED(NORM)                                                                                         \
-  hipLaunchKernelGGL(adam_clipped_kernel<NORM>, dim3((uint32_t)blocks), dim3(kBlock), 0, (hipStream_t)stream, a, types, \
-                     clip, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)bc1,             \
-                     (float)(1.0 / bc2_sqrt), grad_scale)
-  if (norm_type == GSR_NORM_2) GSR_LAUNCH_CLIPPED(GSR_NORM_2);
-  else if (norm_type == GSR_NORM_1) GSR_LAUNCH_CLIPPED(GSR_NORM_1);
-  else GSR_LAUNCH_CLIPPED(GSR_NORM_MAX);
-#undef GSR_LAUNCH_CLIPPED
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kBlock), 0, (hipStream_t)stream, a, types, clip, (float)(1.0 - beta1),
+                       (float)beta2, (float)(1.0 - beta2), (float)eps, (float)bc1, (float)(1.0 / bc2_sqrt), grad_scale);
+  };
+  const bool cached = grad_bytes <= gsr::kLastLevelBytes;
+  if (norm_type == GSR_NORM_2) launch(cached ? adam_clipped_kernel<GSR_NORM_2, true> : adam_clipped_kernel<GSR_NORM_2, false>);
+  else if (norm_type == GSR_NORM_1) launch(cached ? adam_clipped_kernel<GSR_NORM_1, true> : adam_clipped_kernel<GSR_NORM_1, false>);
+  else launch(cached ? adam_clipped_kernel<GSR_NORM_MAX, true> : adam_clipped_kernel<GSR_NORM_MAX, false>);
   return gsr::check_launch("adam_step_clipped");
 }

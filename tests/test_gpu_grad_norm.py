@@ -449,3 +449,15 @@ def test_gradients_beyond_the_last_level_cache():
         check_clipped(t, b, factor64(norm, 0.4 * norm))
         at = 1 + k % 2
         assert torch.equal(p[:at], whole[:at]) and torch.equal(p[at + t.numel():], whole[at + t.numel():])
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 67_108_867), (torch.bfloat16, 134_217_731)])
+def test_a_step_over_gradients_beyond_the_last_level_cache(dtype, n):
+    """Just over 256 MiB of gradients, which the step then reads past the caches: the same bits all the same."""
+    shapes = {"f_rest": (n - 5,), "opacity": (5,)}
+    a, b = make(6, shapes, moments=False), make(6, shapes, moments=False)
+    grads = {k: values(math.prod(s), dtype, j) for j, (k, s) in enumerate(shapes.items())}
+    norm = norm64(grads.values(), 2.0)
+    got = a.step(grads, max_norm=0.3 * norm)
+    b.step({k: g.float() for k, g in grads.items()}, grad_scale=float(np.float32(factor64(norm, 0.3 * norm))))
+    assert abs(float(got) - norm) <= (U + 2.0 ** -25) * norm and same(state_of(a), state_of(b))
