@@ -316,7 +316,9 @@ int launch_clip(int count, const GsrGrad* h_grads, int norm_type, const double* 
   uint64_t chunks = 0;
   for (int k = 0; k < count; k++) chunks += chunks_of(h_grads[k]);
   // Gradients beyond the size of the last-level cache are scaled past it: with the norm pass, 472 MB of fp32 take 236 us
-  // so and 262 through it, 1.4 GB 768 and 821; 165 MB the other way round 80 and 73, 236 MB 111 and 103.
+  // so and 262 through it, 1.4 GB 768 and 821; 165 MB the other way round 80 and 73, 236 MB 111 and 103.  Smaller ones
+  // go through it although buffers that take turns would rather not (118 MB 55 us past it, 64 through it): what reads
+  // them next, as the step does, finds them there (236 MB, clip and step together 391 us past it, 370 through it).
   const bool stream_past = chunks > gsr::kLastLevelBytes / kChunk;
   GradChunks<MOST> a;
   for (int at = 0; at < count;) {
