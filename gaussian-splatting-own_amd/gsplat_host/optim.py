@@ -289,8 +289,9 @@ def clip_grads_(grads: Grads, max_norm: float, norm_type: float = 2.0) -> torch.
 
     Arguments as ``grad_norm``'s; two tensors that share memory, or one that shares it with itself (expanded), are
     refused (only an element that two tensors with gaps between their elements share counts twice and is scaled once).
-    Factor and product are formed in float32 and the product is rounded to the gradient's type.  A NaN norm makes every element NaN and an infinite
-    one the finite elements 0, as there: look at the returned norm, or let ``GaussianAdam.step(skip_nonfinite=True)``.
+    Factor and product are formed in float32 and the product is rounded to the gradient's type.  A NaN norm makes every
+    element NaN and an infinite one the finite elements 0, as there: look at the returned norm, or step with
+    ``GaussianAdam.step(max_norm=..., skip_nonfinite=True)`` instead.
     An infinite ``max_norm`` scales nothing."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
