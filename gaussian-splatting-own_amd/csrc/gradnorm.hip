@@ -131,10 +131,18 @@ __device__ __forceinline__ double add_chunk(double acc, uintptr_t base, uintptr_
   return acc;
 }
 
+// The product of an fp16 element, rounded to fp32 before it is rounded to fp16, as torch's is: left to itself the compiler
+// makes both one mixed-precision instruction that rounds once, which differs where the fp32 product is a tie.
+__device__ __forceinline__ float product_16(float g, float c) {
+  float p = g * c;
+  asm("" : "+v"(p));
+  return p;
+}
+
 template <int TYPE>
 __device__ __forceinline__ uint32_t scale_word(uint32_t w, float c) {
   if (TYPE == GSR_F32) return __float_as_uint(__uint_as_float(w) * c);
-  if (TYPE == GSR_F16) return f32_to_f16(f16_to_f32(w & 0xffffu) * c) | f32_to_f16(f16_to_f32(w >> 16) * c) << 16;
+  if (TYPE == GSR_F16) return f32_to_f16(product_16(f16_to_f32(w & 0xffffu), c)) | f32_to_f16(product_16(f16_to_f32(w >> 16), c)) << 16;
   return f32_to_bf16(__uint_as_float(w << 16) * c) | f32_to_bf16(__uint_as_float(w & 0xffff0000u) * c) << 16;
 }
 
@@ -167,7 +175,7 @@ __device__ __forceinline__ void scale_chunk(float c, uintptr_t base, uintptr_t b
     const uintptr_t a = mine + (uintptr_t)r * kBlock * 16;
     if (a < end && (a < begin || a + 16 > end))
       for (uintptr_t e = a < begin ? begin : a; e < a + 16 && e < end; e += Elem<TYPE>::kSize)
-        Elem<TYPE>::store(e, Elem<TYPE>::load(e) * c);
+        Elem<TYPE>::store(e, TYPE == GSR_F16 ? product_16(Elem<TYPE>::load(e), c) : Elem<TYPE>::load(e) * c);
   }
 }
 
@@ -238,6 +246,18 @@ __global__ void __launch_bounds__(64) norm_final_kernel(const double* __restrict
   if (threadIdx.x == 0) *norm = (float)n;
 }
 
+// The same factor for 16-bit elements, in fp32 as torch forms `max_norm / (norm + 1e-6)`: the reciprocal of the sum,
+// times the bound, each rounded.  bf16 has 128 significands, fp16 1024, and a factor like 0.37 puts whole classes of them
+// on rounding ties (175 * 0.37 = 64.75), so that one last bit of it moves every element of a class the same way and the
+// next norm with them; with torch's bits the results are torch's, bit for bit.  fp32 elements have no such classes: they
+// take the factor rounded once from 64 bits, as the clipped step does.  A norm beyond fp32 has that one only.
+__device__ __forceinline__ float clip_coefficient_16(double norm, double max_norm) {
+  const float n = (float)norm;
+  if (n == __builtin_inff() || max_norm == __builtin_inf()) return gsr::clip_coefficient(norm, max_norm);
+  const float c = 1.0f / (n + 1e-6f) * (float)max_norm;
+  return c < 1.0f || c != c ? c : 1.0f;
+}
+
 // Walks the chunks backwards, eight by eight: what the norm pass read last is still in the last-level cache, and
 // chunk c falls to a workgroup of number c mod 8 in both passes, the same XCD, whose L2 may hold it.  With the norm pass,
 // 1.4 GB / 236 MB / 24 MB: 814 / 107 / 13.9 us forwards, 795 / 106 / 17.2 backwards one by one, 782 / 102 / 13.9 so.
@@ -246,8 +266,8 @@ __global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks<MOST> a, const 
                                                       double max_norm, float* __restrict__ norm, int stream) {
   const double n = gsr::norm_of_partials<NORM>(partials, used);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-  const float coefficient = gsr::clip_coefficient(n, max_norm);
-  if (coefficient == 1.0f) return;                           // x * 1 is x: nothing to write
+  const float c32 = gsr::clip_coefficient(n, max_norm), c16 = clip_coefficient_16(n, max_norm);
+  if (c32 == 1.0f && c16 == 1.0f) return;                    // x * 1 is x: nothing to write
   __shared__ GradChunk s_t[MOST];
   const GradChunk* t = stage(a, s_t);
   const uint32_t eights = (a.chunks + 7) / 8;
@@ -256,6 +276,8 @@ __global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks<MOST> a, const 
     const uint32_t c = (eights - 1 - i / 8) * 8 + i % 8;
     if (c >= a.chunks) continue;
     if (t[k].first > c) k = tensor_of(t, k, c);              // one of those before
+    const float coefficient = t[k].type == GSR_F32 ? c32 : c16;
+    if (coefficient == 1.0f) continue;
     const uintptr_t begin = t[k].begin, end = t[k].end;
     const uintptr_t base = (begin & ~(uintptr_t)15) + (uintptr_t)(c - t[k].first) * kChunk;
     switch (t[k].type + (stream ? 4u : 0u)) {

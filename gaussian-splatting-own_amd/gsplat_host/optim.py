@@ -289,7 +289,9 @@ def clip_grads_(grads: Grads, max_norm: float, norm_type: float = 2.0) -> torch.
 
     Arguments as ``grad_norm``'s; two tensors that share memory, or one that shares it with itself (expanded), are
     refused (only an element that two tensors with gaps between their elements share counts twice and is scaled once).
-    Factor and product are formed in float32 and the product is rounded to the gradient's type.  A NaN norm makes every
+    The product is formed in float32 and rounded to the gradient's type.  The factor of float32 gradients is formed in 64
+    bits and rounded once; float16 and bfloat16 ones take torch's, ``(norm + 1e-6).reciprocal() * max_norm`` in float32
+    throughout, and with it torch's roundings, element by element.  A NaN norm makes every
     element NaN and an infinite one the finite elements 0, as there: look at the returned norm, or step with
     ``GaussianAdam.step(max_norm=..., skip_nonfinite=True)`` instead.
     An infinite ``max_norm`` scales nothing."""

@@ -517,11 +517,14 @@ int gsr_adam_step(int count, const GsrAdamTensor* h_tensors, double beta1, doubl
  * magnitude; 0 without elements, NaN if any element is NaN.  Sums are held in 64 bits;
  * their order depends on the sizes and alignments only, so equal calls give equal bits.
  * gsr_clip_grads: the same norm, and every element times min(1, max_norm / (norm + 1e-6)),
- * the factor and the product in fp32 and the product rounded to its type (the rule of
- * torch.nn.utils.clip_grad_norm_: a NaN norm makes every element NaN, an infinite one makes
- * infinite elements NaN and the others 0).  The factor comes from the 64-bit norm, so it is
- * right where the fp32 *norm overflows.  max_norm >= 0; infinity never scales.  Nothing is
- * written where the factor is 1.  Tensors of the list that share memory are refused.
+ * the product in fp32 and rounded to its type (the rule of torch.nn.utils.clip_grad_norm_:
+ * a NaN norm makes every element NaN, an infinite one makes infinite elements NaN and the
+ * others 0).  The factor of fp32 elements is formed in 64 bits and rounded once to fp32.
+ * 16-bit elements take it in fp32 throughout, as torch forms it from the fp32 *norm (the
+ * reciprocal of norm + 1e-6, times the bound), so that they round as torch's do; where that
+ * norm overflows theirs too comes from 64 bits.  max_norm >= 0; infinity never scales.
+ * Nothing is written where the factor is 1.  Tensors of the list that share memory are
+ * refused.
  * scratch: gsr_grad_norm_bytes(count) bytes, its contents do not matter. */
 #define GSR_F32 0
 #define GSR_F16 1
