@@ -138,14 +138,16 @@ class GradArena:
     def zero_(self) -> None:
         self.flat.zero_()
 
+    # The norm is over the views, not over ``flat``: clipping by a NaN norm would leave NaNs in the padding, which clearing
+    # the gradients alone does not reach, and every later norm would be NaN.
     def norm(self, norm_type: float = 2.0) -> torch.Tensor:
-        """``grad_norm`` of all gradients, as one stretch of memory (the padding is zero).  After ``all_reduce``: every
-        rank then holds the same gradients and finds the same norm, without a collective of its own."""
-        return grad_norm(self.flat, norm_type)
+        """``grad_norm`` of all gradients (the padding between them does not count).  After ``all_reduce``: every rank
+        then holds the same gradients and finds the same norm, without a collective of its own."""
+        return grad_norm(self.views, norm_type)
 
     def clip_(self, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
-        """``clip_grads_`` of all gradients; after ``all_reduce``, as ``norm``."""
-        return clip_grads_(self.flat, max_norm, norm_type)
+        """``clip_grads_`` of all gradients (the padding is left as it is); after ``all_reduce``, as ``norm``."""
+        return clip_grads_(self.views, max_norm, norm_type)
 
     def all_reduce(self, group=None, average: bool = True, method: str = "scatter_gather") -> float:
         """Sums the gradients over the ranks of ``group`` (``method``: see _sum_flat_over_ranks; two collectives on
