@@ -140,14 +140,23 @@ class GradArena:
 
     # The norm is over the views, not over ``flat``: clipping by a NaN norm would leave NaNs in the padding, which clearing
     # the gradients alone does not reach, and every later norm would be NaN.
-    def norm(self, norm_type: float = 2.0) -> torch.Tensor:
-        """``grad_norm`` of all gradients (the padding between them does not count).  After ``all_reduce``: every rank
-        then holds the same gradients and finds the same norm, without a collective of its own."""
-        return grad_norm(self.views, norm_type)
+    def norm(self, norm_type: float = 2.0, grad_scale: float = 1.0) -> torch.Tensor:
+        """``grad_norm`` of ``grad_scale`` times all gradients (the padding between them does not count).  After
+        ``all_reduce`` every rank holds the same gradients and finds the same norm, without a collective of its own;
+        they are SUMS over the ranks then, and ``grad_scale`` is the factor that ``all_reduce`` returned."""
+        scale = _positive_scale(grad_scale)
+        norm = grad_norm(self.views, norm_type)
+        return norm if scale == 1.0 else norm.mul_(scale)
 
-    def clip_(self, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
-        """``clip_grads_`` of all gradients (the padding is left as it is); after ``all_reduce``, as ``norm``."""
-        return clip_grads_(self.views, max_norm, norm_type)
+    def clip_(self, max_norm: float, norm_type: float = 2.0, grad_scale: float = 1.0) -> torch.Tensor:
+        """``clip_grads_`` of all gradients (the padding is left as it is) for a step with ``grad_scale``: the norm that is
+        bounded, and returned, is that of ``grad_scale`` times the gradients, which are themselves scaled by
+        ``min(1, max_norm / (grad_scale (norm + 1e-6)))`` and stay without that factor.  After an averaging
+        ``all_reduce``, pass what it returned here and to the step: without it the sum over the ranks is bounded and not
+        the mean.  ``GaussianAdam.step(max_norm=..., grad_scale=...)`` does both at once."""
+        scale = _positive_scale(grad_scale)
+        norm = clip_grads_(self.views, max_norm / scale, norm_type)
+        return norm if scale == 1.0 else norm.mul_(scale)
 
     def all_reduce(self, group=None, average: bool = True, method: str = "scatter_gather") -> float:
         """Sums the gradients over the ranks of ``group`` (``method``: see _sum_flat_over_ranks; two collectives on
@@ -207,6 +216,13 @@ def _norm_code(norm_type: float) -> int:
     if code is None:
         raise ValueError(f"norm_type must be 1, 2 or infinity, got {norm_type}")
     return code
+
+
+def _positive_scale(grad_scale: float) -> float:
+    grad_scale = float(grad_scale)
+    if not 0.0 < grad_scale < math.inf:
+        raise ValueError(f"grad_scale must be positive and finite, got {grad_scale}")
+    return grad_scale
 
 
 class _GradList:
