@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+from bisect import bisect_left, bisect_right
 from dataclasses import dataclass
 from itertools import chain
 from typing import Dict, Iterable, List, Optional, Union
@@ -288,6 +289,48 @@ def _shares_elements(t: torch.Tensor) -> bool:
     return False
 
 
+def _dims(t: torch.Tensor) -> List[tuple]:
+    """(stride in bytes, size) of ``t``'s dimensions, the longest stride first; those of one element left out."""
+    return sorted(((t.stride(d) * t.element_size(), t.size(d)) for d in range(t.dim()) if t.size(d) > 1), reverse=True)
+
+
+def _touches(t: torch.Tensor, begin: int, end: int) -> bool:
+    """Whether any byte of ``t``'s elements, no two of which share memory, lies in [begin, end).
+
+    Such elements lie in the order of their indices, longest stride first, so those that begin before an address are
+    counted dimension by dimension."""
+    dims = _dims(t)
+
+    def begin_before(address: int) -> int:
+        offset, count = address - t.data_ptr(), 0
+        if offset <= 0 or not t.numel():
+            return 0
+        inner = t.numel()
+        for stride, size in dims:
+            inner //= size
+            whole = min(offset // stride, size)              # of them begin and end their inner dimensions before it
+            count += whole * inner
+            if whole == size:
+                return count
+            offset -= whole * stride
+        return count + (offset > 0)
+
+    return begin < end and begin_before(end) > begin_before(begin - t.element_size() + 1)
+
+
+def _any_stretch_touches(packed: Iterable[torch.Tensor], gapped: Iterable[torch.Tensor]) -> bool:
+    """Whether one of ``packed``, each of which fills a stretch of memory, shares an element with one of ``gapped``.
+    (Two of ``packed`` that overlap are the library's to refuse.)"""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in packed if t.numel())
+    begins, ends = [b for b, _ in spans], [e for _, e in spans]
+    for t in gapped:
+        last = t.data_ptr() + sum(stride * (size - 1) for stride, size in _dims(t)) + t.element_size()
+        near = spans[bisect_right(ends, t.data_ptr()):bisect_left(begins, last)]
+        if any(_touches(t, b, e) for b, e in near):
+            return True
+    return False
+
+
 def grad_norm(grads: Grads, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all gradients together, as a float32 scalar on their GPU; nothing waits for it.
 
@@ -306,7 +349,8 @@ def clip_grads_(grads: Grads, max_norm: float, norm_type: float = 2.0) -> torch.
     ``torch.nn.utils.clip_grad_norm_``) and returns the norm they had, a float32 scalar on their GPU.
 
     Arguments as ``grad_norm``'s; two tensors that share memory, or one that shares it with itself (expanded), are
-    refused (only an element that two tensors with gaps between their elements share counts twice and is scaled once).
+    refused, with one exception: two tensors that BOTH have gaps between their elements are not compared, and an element
+    that they share counts twice and is scaled once.
     The product is formed in float32 and rounded to the gradient's type.  The factor of float32 gradients is formed in 64
     bits and rounded once; float16 and bfloat16 ones take torch's, ``(norm + 1e-6).reciprocal() * max_norm`` in float32
     throughout, and with it torch's roundings, element by element.  A NaN norm makes every
@@ -326,6 +370,9 @@ def clip_grads_(grads: Grads, max_norm: float, norm_type: float = 2.0) -> torch.
         for g, copy in zip(tensors, staged):
             if copy is not None and _shares_elements(g):
                 raise ValueError(f"a gradient of shape {tuple(g.shape)} and strides {g.stride()} has elements that may share memory")
+        if _any_stretch_touches([g for g, copy in zip(tensors, staged) if copy is None],
+                                [g for g, copy in zip(tensors, staged) if copy is not None]):
+            raise ValueError("two gradients of the list share memory: one that fills its memory, and one with gaps")
         listed = _GradList([g if copy is None else copy for g, copy in zip(tensors, staged)])
         norm = listed.run("clip_grads", _lib.gsr_clip_grads, code, max_norm)
         for g, copy in zip(tensors, staged):
