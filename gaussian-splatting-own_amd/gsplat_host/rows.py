@@ -53,10 +53,11 @@ def _contiguous(tensors: Sequence[Optional[torch.Tensor]]) -> List[Optional[torc
 
 
 class _Move:
-    """A move of rows, as far as it can be prepared before the number of rows is known; ``to`` launches it."""
+    """A move of rows, as far as it can be prepared before the number of rows is known; ``to`` launches it.
+    ``tensors`` and ``appended`` are ``_contiguous``."""
 
     def __init__(self, tensors: List[torch.Tensor], appended: List[Optional[torch.Tensor]], rows: int, extra: int):
-        self.tensors, self.appended = _contiguous(tensors), _contiguous(appended)     # kept alive until the launch
+        self.tensors, self.appended = tensors, appended                               # kept alive until the launch
         self.tails = [t.shape[1:] for t in self.tensors]
         self.fixed = [(t.data_ptr(), 0 if e is None else e.data_ptr(), math.prod(s) * t.element_size())
                       for t, e, s in zip(self.tensors, self.appended, self.tails)]
@@ -85,7 +86,7 @@ def select_rows(tensors: Sequence[torch.Tensor], index: torch.Tensor) -> List[to
     if count > MAX_ROWS:
         raise ValueError(f"{count} rows: at most {MAX_ROWS}")
     with _dgr._on_device(dev.index):
-        return _Move(tensors, [None] * len(tensors), rows, 0).to(index.contiguous(), count)
+        return _Move(_contiguous(tensors), [None] * len(tensors), rows, 0).to(index.contiguous(), count)
 
 
 _tickets = itertools.count(1)
@@ -142,15 +143,20 @@ def compact_rows(tensors: Sequence[torch.Tensor], keep: torch.Tensor,
     with _dgr._on_device(dev.index):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("compact_rows reads the number of kept rows and cannot be captured into a graph; select_rows can")
-        keep = keep.contiguous()
+        keep, tensors, more = keep.contiguous(), _contiguous(tensors), _contiguous(more)
         nb = _lib.gsr_keep_rows_bytes()
         scratch = torch.empty((nb,), dtype=torch.uint8, device=dev)
         index = torch.empty((total,), dtype=torch.int32, device=dev)
         _, word = _landing(dev)
         ticket = next(_tickets) & 0xFFFFFFFF or next(_tickets) & 0xFFFFFFFF       # never 0
-        _dgr._run("keep_rows", _lib.gsr_keep_rows, total, keep.data_ptr(), index.data_ptr(), C.addressof(word), ticket,
-                  scratch.data_ptr(), nb, _dgr._raw_stream(dev.index))
-        move = _Move(tensors, more, rows, extra)                                  # while the GPU counts
-        count = _await_count(word, ticket, dev)
+        try:
+            _dgr._run("keep_rows", _lib.gsr_keep_rows, total, keep.data_ptr(), index.data_ptr(), C.addressof(word), ticket,
+                      scratch.data_ptr(), nb, _dgr._raw_stream(dev.index))
+            move = _Move(tensors, more, rows, extra)                              # while the GPU counts
+            count = _await_count(word, ticket, dev)
+        except BaseException:
+            # the count may still be under way: it must not land in a later call's word, nor in one that is gone
+            torch.cuda.current_stream(dev).synchronize()
+            raise
         index = index[:count]
         return move.to(index, count), index
