@@ -456,24 +456,40 @@ class GaussianAdam:
     @torch.no_grad()
     def refine(self, keep: torch.Tensor, extension: Optional[Dict[str, torch.Tensor]] = None) -> Dict[str, torch.nn.Parameter]:
         """``cat_tensors(extension)`` and then ``prune(keep)``, in one pass: ``keep`` has one bool per row, the old
-        ones first and the appended ones behind them.  On the GPU all tensors and moments are moved by one launch and
-        the concatenations are never built (``gsplat_host.rows.compact_rows``)."""
+        ones first and the appended ones behind them.  On the GPU the parameters and each of the moments are moved by a
+        launch each and the concatenations are never built (``gsplat_host.rows.compact_rows``).  Arguments that do not fit
+        are refused before anything changes.  Where memory ends between two of the launches the parameters stay as they
+        are and their moments start again at zero."""
         if extension is not None and set(extension) != set(self.params):
             raise ValueError(f"extension must name every tensor: {sorted(self.params)}")
         if not keep.is_cuda:
             if extension is not None:
                 self.cat_tensors(extension)
             return self.prune(keep)
-        from .rows import compact_rows
+        from . import rows
         names = list(self.params)
-        more = None
+        new, nothing = [None] * len(names), [None] * len(names)
         if extension is not None:
-            more = [extension[n].detach().to(self.params[n].dtype) for n in names] + [None] * (2 * len(names))
-        rows, _ = compact_rows([self.params[n].detach() for n in names] + [self.exp_avg[n] for n in names]
-                               + [self.exp_avg_sq[n] for n in names], keep, more)
-        for i, n in enumerate(names):
-            self.params[n] = torch.nn.Parameter(rows[i].requires_grad_(True))
-            self.exp_avg[n], self.exp_avg_sq[n] = rows[len(names) + i], rows[2 * len(names) + i]
+            new = [extension[n].detach().to(self.params[n].dtype) for n in names]
+        groups = (self.exp_avg, self.exp_avg_sq, self.params)
+        _, _, _, _, extra = rows._checked_compaction([g[n].detach() for g in groups for n in names], keep,
+                                                     None if extension is None else nothing + nothing + new)
+        # group by group, so that the old moments go as the new ones come: a third of the state on top of it at the peak
+        # and not all of it (the old parameters are the caller's until it takes the new ones)
+        moved, index = rows.compact_rows([self.exp_avg[n] for n in names], keep, nothing)
+        self.exp_avg.update(zip(names, moved))
+        try:
+            moved = rows._again([self.exp_avg_sq[n] for n in names], index, nothing, extra)
+            self.exp_avg_sq.update(zip(names, moved))
+            moved = rows._again([self.params[n].detach() for n in names], index, new, extra)
+        except BaseException:
+            # the old moments are gone and the parameters are as they were: their moments start again
+            moved = index = None
+            for moments in (self.exp_avg, self.exp_avg_sq):
+                moments.clear()
+                moments.update((n, torch.zeros_like(p)) for n, p in self.params.items())
+            raise
+        self.params.update([(n, torch.nn.Parameter(t.requires_grad_(True))) for n, t in zip(names, moved)])
         return dict(self.params)
 
     @torch.no_grad()

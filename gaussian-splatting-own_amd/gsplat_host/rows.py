@@ -115,15 +115,7 @@ def _await_count(word: C.c_uint64, ticket: int, dev: torch.device) -> int:
     return value & 0xFFFFFFFF
 
 
-def compact_rows(tensors: Sequence[torch.Tensor], keep: torch.Tensor,
-                 appended: Optional[Sequence[Optional[torch.Tensor]]] = None) -> Tuple[List[torch.Tensor], torch.Tensor]:
-    """``([torch.cat((t, a))[keep] for t, a in zip(tensors, appended)], index)`` without the concatenations.
-
-    ``keep``: one bool per row, first the tensors' rows, then the appended ones.  ``appended``: for each tensor the rows
-    behind its own, or None for rows of zeros (the moments of new Gaussians); None altogether: nothing is appended.
-    ``index`` (int32): the positions of the kept rows, so ``index[j]`` is where row j of the results came from.
-    The order stays.  The number of kept rows sizes the results, so the host waits for it and the call cannot be
-    captured into a graph."""
+def _checked_compaction(tensors: Sequence[torch.Tensor], keep: torch.Tensor, appended: Optional[Sequence[Optional[torch.Tensor]]]):
     tensors, dev, rows = _checked(tensors)
     if keep.dtype != torch.bool or keep.dim() != 1:
         raise TypeError(f"keep must be a one-dimensional bool tensor, got {keep.dtype} of shape {tuple(keep.shape)}")
@@ -140,6 +132,26 @@ def compact_rows(tensors: Sequence[torch.Tensor], keep: torch.Tensor,
         if e is not None and (e.shape != (extra, *t.shape[1:]) or e.dtype != t.dtype or e.device != dev or e.layout != torch.strided):
             raise ValueError(f"appended rows of shape {tuple(e.shape)}, {e.dtype} on {e.device} do not fit {extra} rows of a "
                              f"tensor of shape {tuple(t.shape)}, {t.dtype} on {dev}")
+    return tensors, more, dev, rows, extra
+
+
+def _again(tensors: Sequence[torch.Tensor], index: torch.Tensor, appended: Sequence[Optional[torch.Tensor]], extra: int) -> List[torch.Tensor]:
+    """The rows of more ``tensors`` that a ``compact_rows`` with the same numbers of rows kept; arguments have been checked."""
+    with _dgr._on_device(index.get_device()):
+        return _Move(_contiguous(tensors), _contiguous(appended), tensors[0].shape[0], extra).to(index, index.numel())
+
+
+def compact_rows(tensors: Sequence[torch.Tensor], keep: torch.Tensor,
+                 appended: Optional[Sequence[Optional[torch.Tensor]]] = None) -> Tuple[List[torch.Tensor], torch.Tensor]:
+    """``([torch.cat((t, a))[keep] for t, a in zip(tensors, appended)], index)`` without the concatenations.
+
+    ``keep``: one bool per row, first the tensors' rows, then the appended ones.  ``appended``: for each tensor the rows
+    behind its own, or None for rows of zeros (the moments of new Gaussians); None altogether: nothing is appended.
+    ``index`` (int32): the positions of the kept rows, so ``index[j]`` is where row j of the results came from.
+    The order stays.  The number of kept rows sizes the results, so the host waits for it and the call cannot be
+    captured into a graph."""
+    tensors, more, dev, rows, extra = _checked_compaction(tensors, keep, appended)
+    total = rows + extra
     with _dgr._on_device(dev.index):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("compact_rows reads the number of kept rows and cannot be captured into a graph; select_rows can")
