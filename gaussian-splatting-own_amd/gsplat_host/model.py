@@ -142,6 +142,12 @@ class GaussianParams(nn.Module):
         self.denom = torch.zeros((n, 1), device=dev)
         self.max_radii2D = torch.zeros((n,), device=dev)
 
+    def _refines_in_one_pass(self) -> bool:
+        """Whether append and prune may be one ``optimizer.refine``: the optimiser has it (``prune`` and ``cat_tensors`` are
+        enough for the two steps), and no subclass does more in them or reads its parameters in another way."""
+        steps = ("densification_postfix", "prune_points", "get_opacity", "get_scaling")
+        return hasattr(self.optimizer, "refine") and all(getattr(type(self), s) is getattr(GaussianParams, s) for s in steps)
+
     @torch.no_grad()
     def densify_and_prune(self, max_grad, min_opacity, extent, max_screen_size, generator=None, children: int = 2) -> None:
         """The refinement step train.py:118-120 runs every 100 iterations, with the rules of
@@ -185,15 +191,20 @@ class GaussianParams(nn.Module):
         born["scaling"][copies:] = torch.log(spread / (0.8 * children))
 
         appended = source.numel()
+        in_one_pass = appended and self._refines_in_one_pass()
+        if appended and not in_one_pass:
+            self.densification_postfix(*(born[g] for g in ("xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation")))
         total = count + appended
         gone = torch.zeros((total,), dtype=torch.bool, device=dev)
         gone[parent_idx] = True
-        gone |= torch.sigmoid(torch.cat((self._opacity, born["opacity"]))).reshape(-1) < min_opacity
+        opacity = torch.sigmoid(torch.cat((self._opacity, born["opacity"]))) if in_one_pass else self.get_opacity
+        gone |= opacity.reshape(-1) < min_opacity
         if max_screen_size:
-            gone |= torch.exp(torch.cat((self._scaling, born["scaling"]))).amax(dim=1) > 0.1 * extent
+            scale = torch.exp(torch.cat((self._scaling, born["scaling"]))) if in_one_pass else self.get_scaling
+            gone |= scale.amax(dim=1) > 0.1 * extent
             if not appended:                                    # an append starts the recorded radii again, as in the reference
                 gone |= self.max_radii2D > max_screen_size
-        if not appended:
+        if not in_one_pass:
             self.prune_points(gone)
             return
         self._adopt(self.optimizer.refine(~gone, born))

@@ -440,7 +440,7 @@ class GaussianAdam:
         """_prune_optimizer (:273-289): keeps the rows selected by the boolean mask ``keep`` of every tensor and
         of both moments; returns the new parameters by group name."""
         if self._moves_rows_on_the_gpu(keep):
-            return self.refine(keep, None)
+            return self._move_rows(keep, None)
         for name, p in self.params.items():
             self.exp_avg[name] = self.exp_avg[name][keep].contiguous()
             self.exp_avg_sq[name] = self.exp_avg_sq[name][keep].contiguous()
@@ -462,10 +462,15 @@ class GaussianAdam:
         are and their moments start again at zero."""
         if extension is not None and set(extension) != set(self.params):
             raise ValueError(f"extension must name every tensor: {sorted(self.params)}")
-        if not keep.is_cuda:
-            if extension is not None:
-                self.cat_tensors(extension)
-            return self.prune(keep)
+        own_steps = type(self).prune is GaussianAdam.prune and type(self).cat_tensors is GaussianAdam.cat_tensors
+        if keep.is_cuda and own_steps:
+            return self._move_rows(keep, extension)
+        if extension is not None:                  # a subclass may do more in these
+            self.cat_tensors(extension)
+        return self.prune(keep)
+
+    def _move_rows(self, keep: torch.Tensor, extension: Optional[Dict[str, torch.Tensor]]) -> Dict[str, torch.nn.Parameter]:
+        """``refine`` on the GPU."""
         from . import rows
         names = list(self.params)
         new, nothing = [None] * len(names), [None] * len(names)
