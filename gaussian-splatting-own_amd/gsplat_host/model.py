@@ -202,8 +202,9 @@ class GaussianParams(nn.Module):
         if max_screen_size:
             scale = torch.exp(torch.cat((self._scaling, born["scaling"]))) if in_one_pass else self.get_scaling
             gone |= scale.amax(dim=1) > 0.1 * extent
-            if not appended:                                    # an append starts the recorded radii again, as in the reference
-                gone |= self.max_radii2D > max_screen_size
+            # an append starts the recorded radii again, as in the reference
+            radii = torch.zeros((total,), device=dev) if in_one_pass else self.max_radii2D
+            gone |= radii > max_screen_size
         if not in_one_pass:
             self.prune_points(gone)
             return
