@@ -465,6 +465,16 @@ class GaussianAdam:
         own_steps = type(self).prune is GaussianAdam.prune and type(self).cat_tensors is GaussianAdam.cat_tensors
         if keep.is_cuda and own_steps:
             return self._move_rows(keep, extension)
+        extra = 0
+        for n, p in self.params.items():           # nothing has been appended when a call is refused
+            if extension is not None:
+                extra = next(iter(extension.values())).shape[0]
+                if extension[n].shape != (extra, *p.shape[1:]):
+                    raise ValueError(f"{n}: appended rows of shape {tuple(extension[n].shape)} do not fit {extra} rows of a "
+                                     f"tensor of shape {tuple(p.shape)}")
+            if keep.dtype != torch.bool or keep.shape != (p.shape[0] + extra,):
+                raise ValueError(f"keep must have a bool for each of {p.shape[0]} + {extra} rows, got {keep.dtype} of shape "
+                                 f"{tuple(keep.shape)}")
         if extension is not None:                  # a subclass may do more in these
             self.cat_tensors(extension)
         return self.prune(keep)
