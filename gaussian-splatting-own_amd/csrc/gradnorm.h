@@ -2,6 +2,7 @@
 #pragma once
 
 #include "gsr_common.h"
+#include "plan.h"
 
 namespace gsr {
 
@@ -10,8 +11,6 @@ constexpr int kNormBlocks = 512;
 // Partial results that every clipping wave joins by itself; more of them (over 480 tensors) are joined by a kernel of
 // their own first, which costs a launch (4 us) but not their reading by every wave.
 constexpr int kMostJoined = 4 * kNormBlocks;
-// What of the gradients the pass leaves in the last-level cache, for those that come to them next.
-constexpr uint64_t kLastLevelBytes = 256ull << 20;
 // Descriptors that fit one launch's kernel arguments (4 KB).
 constexpr int kGradsPerLaunch = 120;
 

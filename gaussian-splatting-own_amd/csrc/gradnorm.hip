@@ -22,6 +22,7 @@ namespace {
 using gsr::global_at;
 using gsr::kGradsPerLaunch;
 using gsr::kNormBlocks;
+using gsr::size_of;
 
 // 1.4 GB and 236 MB of fp32, norm alone: 230 and 37.6 us with 512 workgroups (kNormBlocks) of 512 threads and four
 // accesses in flight; 1024 workgroups 237 / 40, 256 of them 265 / 37.5; 1024 workgroups of 256 threads 233 / 40, 256 of
@@ -291,8 +292,6 @@ __global__ void __launch_bounds__(kBlock) clip_kernel(GradChunks<MOST> a, const 
   }
 }
 
-inline size_t size_of(uint64_t type) { return type == GSR_F32 ? 4 : 2; }
-
 inline uint64_t chunks_of(const GsrGrad& g) {
   if (!g.n) return 0;
   const uintptr_t begin = (uintptr_t)g.grad;
@@ -335,13 +334,11 @@ int launch_norm(int count, const GsrGrad* h_grads, int norm_type, double* partia
 template <int MOST>
 int launch_clip(int count, const GsrGrad* h_grads, int norm_type, const double* partials, int used, double max_norm,
                 float* norm, hipStream_t stream) {
-  uint64_t chunks = 0;
-  for (int k = 0; k < count; k++) chunks += chunks_of(h_grads[k]);
   // Gradients beyond the size of the last-level cache are scaled past it: with the norm pass, 472 MB of fp32 take 236 us
   // so and 262 through it, 1.4 GB 768 and 821; 165 MB the other way round 80 and 73, 236 MB 111 and 103.  Smaller ones
   // go through it although buffers that take turns would rather not (118 MB 55 us past it, 64 through it): what reads
   // them next, as the step does, finds them there (236 MB, clip and step together 391 us past it, 370 through it).
-  const bool stream_past = chunks > gsr::kLastLevelBytes / kChunk;
+  const bool stream_past = gsr::past_last_level(count, h_grads);
   GradChunks<MOST> a;
   for (int at = 0; at < count;) {
     fill(a, count, h_grads, &at);

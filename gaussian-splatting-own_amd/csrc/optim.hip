@@ -265,11 +265,10 @@ extern "C" int gsr_adam_step_clipped(int count, const GsrAdamTensor* h_tensors, 
   if (rc != GSR_OK) return rc;
   AdamTensors a{};
   GradTypes types{};
-  uint64_t blocks = 0, grad_bytes = 0;
+  uint64_t blocks = 0;
   for (int k = 0; k < count; k++) {
     const GsrAdamTensor& t = h_tensors[k];
     if (t.n == 0) continue;
-    grad_bytes += t.n * (grads[k].type == GSR_F32 ? 4 : 2);
     GsrAdamTensor u = t;
     const uintptr_t grad_align = grads[k].type == GSR_F32 ? 15 : 7;
     u.vec4 = (((uintptr_t)t.param | (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) & 15) == 0 && ((uintptr_t)t.grad & grad_align) == 0;
@@ -291,7 +290,7 @@ extern "C" int gsr_adam_step_clipped(int count, const GsrAdamTensor* h_tensors, 
     hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(kBlock), 0, (hipStream_t)stream, a, types, clip, (float)(1.0 - beta1),
                        (float)beta2, (float)(1.0 - beta2), (float)eps, (float)bc1, (float)(1.0 / bc2_sqrt), grad_scale);
   };
-  const bool cached = grad_bytes <= gsr::kLastLevelBytes;
+  const bool cached = !gsr::past_last_level(count, grads);
   if (norm_type == GSR_NORM_2) launch(cached ? adam_clipped_kernel<GSR_NORM_2, true> : adam_clipped_kernel<GSR_NORM_2, false>);
   else if (norm_type == GSR_NORM_1) launch(cached ? adam_clipped_kernel<GSR_NORM_1, true> : adam_clipped_kernel<GSR_NORM_1, false>);
   else launch(cached ? adam_clipped_kernel<GSR_NORM_MAX, true> : adam_clipped_kernel<GSR_NORM_MAX, false>);
