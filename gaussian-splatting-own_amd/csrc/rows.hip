@@ -14,8 +14,13 @@
 #include <algorithm>
 
 #include "gsr_common.h"
+#include "plan.h"
 
 namespace {
+
+using gsr::Divisor;
+using gsr::divisor;
+using gsr::lies_in_two_rows;
 
 constexpr int kBlock = 256;
 // Vectors of a thread, a block's width apart.  Everything is read and written once, so the accesses are nontemporal.
@@ -24,17 +29,6 @@ constexpr int kBlock = 256;
 constexpr int kRounds = 2;
 constexpr int kPerBlock = kBlock * kRounds;        // vectors of 16 bytes
 constexpr int kRowsPerLaunch = 48;                 // descriptors that fit the kernel arguments
-
-// n / d for every 32-bit n by a multiplication (Granlund and Montgomery 1994, the round-up method): with
-// l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1, q = (t + ((n - t) >> 1)) >> (l - 1), t = mulhi(m, n); d > 1.
-struct Divisor {
-  uint32_t d, m, shift;
-  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
-    if (d == 1) return n;
-    const uint32_t t = __umulhi(m, n);
-    return (t + ((n - t) >> 1)) >> shift;
-  }
-};
 
 struct Moves {
   struct One {
@@ -124,13 +118,6 @@ __device__ __forceinline__ void move_block(const Moves& a, const Moves::One& t, 
     const uint32_t over = t.units.quotient(col0 + at);
     move_units<U, I>(a, t, first + at, total, row0 + over, col0 + at - over * t.units.d);
   }
-}
-
-// Whether a vector, which begins at a multiple of K units of the output, never reaches into a third row: column and
-// length together stay below two rows.  All rows of 15 bytes and more, and those that divide a vector in half.
-inline bool lies_in_two_rows(uint32_t units, uint32_t unit) {
-  const uint32_t k = 16 / unit;
-  return units + k - 2 < 2 * units || 2 * units == k;
 }
 
 // The same for rows that lies_in_two_rows holds for, the ordinary case.  One wide load from where the vector begins,
@@ -284,17 +271,6 @@ __global__ void __launch_bounds__(kBlock) keep_write_kernel(Flags f, const uint3
 constexpr uint64_t kMostRows = 0x7fff0000ull;      // row numbers are 32-bit signed, with room to round up
 
 constexpr uint64_t kMostMoveBlocks = 0xffffffull;  // a launch has fewer than 2^32 threads: 137 GB of rows
-
-Divisor divisor(uint32_t d) {
-  Divisor v = {d, 0, 0};
-  if (d > 1) {
-    uint32_t l = 0;
-    while ((1ull << l) < d) l++;
-    v.m = (uint32_t)(((((uint64_t)1 << l) - d) << 32) / d + 1);
-    v.shift = l - 1;
-  }
-  return v;
-}
 
 }  // namespace
 
