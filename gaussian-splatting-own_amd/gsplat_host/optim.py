@@ -602,7 +602,8 @@ class GaussianAdam:
                 raise ValueError(f"{name}: gradient has {g.numel()} elements, parameter {n}")
             if n == 0:
                 continue
-            g = g.resolve_neg()                    # a negated view's memory holds the opposite of its values
+            if g.is_neg():                         # a negated view's memory holds the opposite of its values
+                g = g.resolve_neg()
             if max_norm is None:
                 g = _dgr._f32(g, f"grad of {name}")
             else:
