@@ -11,7 +11,8 @@ constexpr int kNormBlocks = 512;
 // Partial results that every clipping wave joins by itself; more of them (over 480 tensors) are joined by a kernel of
 // their own first, which costs a launch (4 us) but not their reading by every wave.
 constexpr int kMostJoined = 4 * kNormBlocks;
-// Descriptors that fit one launch's kernel arguments (4 KB).
+// Descriptors of a launch: 24 bytes each, 2.9 KB of kernel arguments, which every launch copies.  A choice, not a limit
+// that was found: more of them a launch have not been measured.
 constexpr int kGradsPerLaunch = 120;
 
 // Writes the partial results of all gradients to `partials` (norm_partials_most(count) doubles) and their number to
