@@ -469,9 +469,9 @@ class GaussianAdam:
         for n, p in self.params.items():           # nothing has been appended when a call is refused
             if extension is not None:
                 extra = next(iter(extension.values())).shape[0]
-                if extension[n].shape != (extra, *p.shape[1:]):
-                    raise ValueError(f"{n}: appended rows of shape {tuple(extension[n].shape)} do not fit {extra} rows of a "
-                                     f"tensor of shape {tuple(p.shape)}")
+                if extension[n].shape != (extra, *p.shape[1:]) or extension[n].device != p.device:
+                    raise ValueError(f"{n}: appended rows of shape {tuple(extension[n].shape)} on {extension[n].device} do not "
+                                     f"fit {extra} rows of a tensor of shape {tuple(p.shape)} on {p.device}")
             if keep.dtype != torch.bool or keep.shape != (p.shape[0] + extra,):
                 raise ValueError(f"keep must have a bool for each of {p.shape[0]} + {extra} rows, got {keep.dtype} of shape "
                                  f"{tuple(keep.shape)}")

@@ -19,3 +19,12 @@ def test_nothing_is_appended_by_a_refused_call():
         assert all(a[n] is b[n] for a, b in zip(held, (opt.params, opt.exp_avg, opt.exp_avg_sq)) for n in SHAPES)
     opt.refine(keep, good)
     assert opt.params["xyz"].shape[0] == 44
+
+
+def test_rows_on_another_device_are_refused_first():
+    opt = GaussianAdam({k: torch.randn(*s) for k, s in SHAPES.items()}, dict.fromkeys(SHAPES, 0.1))
+    held = [dict(d) for d in (opt.params, opt.exp_avg, opt.exp_avg_sq)]
+    born = {k: torch.zeros(4, *s[1:], device="meta" if k == "opacity" else "cpu") for k, s in SHAPES.items()}
+    with pytest.raises(ValueError, match="on meta"):
+        opt.refine(torch.ones(44, dtype=torch.bool), born)
+    assert all(a[n] is b[n] for a, b in zip(held, (opt.params, opt.exp_avg, opt.exp_avg_sq)) for n in SHAPES)
